@@ -219,14 +219,14 @@ def run(s):
             rows, residual = ops.fused_add_rms_norm_mx(s["x"], s["residual"], s["gain"], EPS)
             return [rows.q, rows.s, residual]
         if kind == "linear":
-            return [ops.mx_linear(s["x"], *s["weight"], s["bias"])]
+            return [ops.mx_linear(s["x"], s["weight"], s["bias"])]
         if kind == "normed":
             rows, residual = ops.fused_add_rms_norm_mx(s["x"], s["residual"], s["gain"], EPS)
-            return [ops.mx_linear(rows, *s["weight"], s["bias"]), residual]
+            return [ops.mx_linear(rows, s["weight"], s["bias"]), residual]
         if kind == "gate_up":
-            rows = ops.mx_gate_up(s["x"], *s["weight"])
+            rows = ops.mx_gate_up(s["x"], s["weight"])
             return [rows.q, rows.s]
-        return [ops.mx_experts(s["x"], s["topw"], s["topi"], *s["weight13"], *s["weight2"], s["bias13"], s["b2"], limit=s["limit"])]
+        return [ops.mx_experts(s["x"], s["topw"], s["topi"], s["weight13"], s["weight2"], s["bias13"], s["b2"], limit=s["limit"])]
     x = s["x"].float()
     if kind == "quantize":
         if s["bits"] == 8:
