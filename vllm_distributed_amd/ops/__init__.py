@@ -12,7 +12,8 @@ from typing import Optional, Tuple
 import torch
 
 from .. import envs
-from . import torch_ref
+from . import quant, torch_ref
+from .quant import MxRows, MxWeight  # noqa: F401
 from .torch_ref import k_cache_shape, v_cache_shape  # noqa: F401  (the paged-cache layouts every backend shares)
 
 # rows up to which a projection may leave fp32 partial sums of a split K to the kernel that follows
@@ -483,6 +484,129 @@ def fp4_linear(x, qw, fs, alpha=None, bias=None, dense=None):
     if bias is not None:
         y = y + bias
     return y.view(shape[:-1] + (y.shape[-1],))
+
+
+# ------------------------------------------------------------------ microscaled formats: blocks of 32 values, one power of two each
+def _mx_hip(t: torch.Tensor, dtype: torch.dtype) -> bool:
+    return _use_hip(t) and dtype in (torch.bfloat16, torch.float16)
+
+
+def _mx_width(k: int) -> None:
+    if k <= 0 or k % 32:
+        raise ValueError(f"{k} columns are not whole blocks of 32")
+
+
+def mx_quantize(x, bits: int = 8) -> MxRows:
+    """Rows ``x [.., K]`` (16- or 32-bit floats, ``K % 32 == 0``) in microscaled floating point: elements of 8 (e4m3) or 4 (e2m1) bits,
+    a power of two for each 32 neighbours - the smallest that keeps every element within the format, so none saturates; elements
+    to nearest, ties to even.  A block with a NaN or an infinity becomes NaN as a whole."""
+    if bits not in (4, 8):
+        raise ValueError(f"microscaled rows hold 8 or 4 bits a value, not {bits}")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"mx_quantize of {x.dtype}")
+    _mx_width(x.shape[-1])
+    x2 = x.reshape(-1, x.shape[-1])
+    return _hip.mx_quantize(x2, bits) if _use_hip(x2) else quant.mx_quantize(x2, bits)
+
+
+def mx_dequantize(rows: MxRows, dtype: Optional[torch.dtype] = None):
+    """The numbers that ``rows`` stand for, ``[M, K]`` in ``dtype`` (``rows.dtype``), rounded once."""
+    dtype = dtype or rows.dtype
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"mx_dequantize to {dtype}")
+    return _hip.mx_dequantize(rows, dtype) if _use_hip(rows.payload) else quant.mx_dequantize(rows, dtype)
+
+
+def rms_norm_mx(x, weight, eps) -> MxRows:
+    """``rms_norm`` whose result leaves as 8-bit microscaled rows (``x [.., H]``, ``H % 32 == 0``)."""
+    _mx_width(weight.numel())
+    if _mx_hip(x, x.dtype):
+        return _hip.mx_rms_norm(x, None, None, weight, eps)[0]
+    return torch_ref.rms_norm_mx(x, None, weight, eps)[0]
+
+
+def fused_add_rms_norm_mx(x, residual, weight, eps) -> Tuple[MxRows, torch.Tensor]:
+    """``(rms_norm(x + residual) * weight as 8-bit microscaled rows, x + residual rounded to its type)``.  The norm is taken of the
+    32-bit sum; ``x`` and ``residual`` stay as they are."""
+    _mx_width(weight.numel())
+    if _mx_hip(residual, residual.dtype):
+        return _hip.mx_rms_norm(x, None, residual, weight, eps)
+    return torch_ref.rms_norm_mx(x, residual, weight, eps)
+
+
+def reduce_add_rms_norm_mx(partial, residual, weight, eps) -> Tuple[MxRows, torch.Tensor]:
+    """``fused_add_rms_norm_mx`` whose first operand arrives as fp32 K-split slabs ``[ks, T, H]``."""
+    _mx_width(weight.numel())
+    if _mx_hip(residual, residual.dtype):
+        return _hip.mx_rms_norm(None, partial, residual, weight, eps)
+    return torch_ref.rms_norm_mx(partial.sum(0), residual, weight, eps)
+
+
+def _mx_operand(x, w: MxWeight) -> MxRows:
+    """``x`` (16-bit rows, quantised here, or rows that are 8-bit already) as the left operand of a product with ``w``."""
+    rows = x if isinstance(x, MxRows) else mx_quantize(x, 8)
+    if rows.bits != 8:
+        raise ValueError("products take 8-bit microscaled rows")
+    if (rows.width + 127) // 128 != w.qw.shape[-3]:
+        raise ValueError(f"rows of {rows.width} columns and a weight of {w.qw.shape[-3] * 128} (padded)")
+    return rows
+
+
+def mx_linear(x, weight: MxWeight, bias=None):
+    """``y = x W^T (+ bias)`` for a 4-bit microscaled weight (``ops.quant.pack_mx``) and rows in 8 bits (``x``: an ``MxRows``, or 16-bit
+    rows that are quantised here), on the scaled matrix instructions with 32-bit sums."""
+    rows = _mx_operand(x, weight)
+    if _mx_hip(rows.payload, rows.dtype):
+        y = _hip.mx_linear(rows, weight, bias)
+    else:
+        y = quant.mx_product(rows, weight, bias).to(rows.dtype)
+    return y if isinstance(x, MxRows) else y.view(x.shape[:-1] + (y.shape[-1],))
+
+
+def mx_linear_partials(x, weight: MxWeight):
+    """``mx_linear`` without a bias left as fp32 K-split slabs ``[ks, M, N]`` for the norm or the rotary kernel that follows; None where
+    the product runs unsplit."""
+    if not (_use_hip(x.payload if isinstance(x, MxRows) else x) and envs.VDAMD_FUSED_REDUCE_NORM):
+        return None
+    rows = _mx_operand(x, weight)
+    return _hip.mx_linear_partials(rows, weight) if rows.dtype in (torch.bfloat16, torch.float16) else None
+
+
+def mx_gate_up(x, weight: MxWeight, bias=None, limit: float = 0.0, alpha: float = 1.702) -> MxRows:
+    """``silu(x Wg^T) * (x Wu^T)`` as 8-bit microscaled rows for ``weight = [Wg ; Wu]`` (``pack_mx(..., halves=2)``: halves of whole 128
+    rows).  ``limit`` > 0: gpt-oss' clamped form ``(clamp(u) + 1) g sigmoid(alpha g)``, ``g`` clamped from above.  The activation is
+    formed and quantised from the 32-bit sums."""
+    rows = _mx_operand(x, weight)
+    if weight.rows % 256:
+        raise ValueError(f"{weight.rows} rows of gate and up: halves of whole 128 are wanted (pack_mx with halves=2)")
+    if _mx_hip(rows.payload, rows.dtype):
+        return _hip.mx_gate_up(rows, weight, bias, limit, alpha)
+    return quant.mx_quantize(quant.mx_gated(quant.mx_product(rows, weight, bias), limit, alpha), 8, rows.dtype)
+
+
+def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None, bias2=None, expert_start: int = 0,
+               local_experts: int = -1, num_experts: int = 0, limit: float = 0.0, alpha: float = 1.702):
+    """A sparse block behind its router: ``sum_j topw[t, j] down_e(gated_e(x[t]))``, ``e = topi[t, j]``, for experts whose matrices are
+    4-bit microscaled (``weight13`` ``[E, gate ; up]`` packed with ``halves=2``, ``weight2 [E, H]``) with biases ``[E, rows]``.  ``x [T, H]``
+    16-bit rows or an ``MxRows``, ``topw [T, k]`` fp32, ``topi [T, k]`` int32.  ``expert_start`` / ``local_experts`` (expert parallel): the
+    matrices are those of experts ``expert_start ..``, other slots add nothing; ``num_experts``: the router's outputs then."""
+    e_local = weight13.qw.shape[0]
+    total = num_experts or (e_local if local_experts < 0 else expert_start + local_experts)
+    rows = _mx_operand(x, weight13)
+    t, k = topi.shape
+    if rows.shape[0] != t or topw.shape != topi.shape:
+        raise ValueError(f"{rows.shape[0]} rows, choices {tuple(topi.shape)}, weights {tuple(topw.shape)}")
+    if local_experts >= 0 and not num_experts:
+        raise ValueError("the number of the router's outputs is wanted beside local_experts")
+    if local_experts >= 0 and local_experts != e_local or weight2.qw.shape[0] != e_local:
+        raise ValueError(f"{e_local} and {weight2.qw.shape[0]} expert matrices, {local_experts} local experts")
+    if _mx_hip(rows.payload, rows.dtype) and t:
+        tile_rows = _hip.mx_tile_rows(t * k, total)
+        src_row, inv, tiles = moe_align_fused(topi, total, tile_rows, expert_start, local_experts)
+        a = _hip.mx_grouped_gate_up(rows, weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
+        y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2)
+        return moe_combine(y, topw, topi, inv, expert_start, local_experts)
+    return torch_ref.mx_experts(rows, topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)
 
 
 def moe_align(topi, num_experts: int, tile_rows: int, expert_start: int = 0, local_experts: int = -1):

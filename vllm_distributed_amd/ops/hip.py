@@ -17,6 +17,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..logger import init_logger
+from . import quant
 
 logger = init_logger(__name__)
 _LIB: Optional[ctypes.CDLL] = None
@@ -95,6 +96,10 @@ def load() -> ctypes.CDLL:
         "vdamd_delta_rule_rows": [P, P, L, P, L, P, L] + [P] * 6 + [I] * 6 + [F, I, P],
         "vdamd_gated_delta_rule": [P, P, L, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
         "vdamd_embed_scaled": [P, P, P, F, I, I, I, I, P],
+        "vdamd_mx_quantize": [P, L, P, L, P, L, L, I, I, I, I, P],
+        "vdamd_mx_dequantize": [P, P, L, P, L, L, I, I, I, P],
+        "vdamd_mx_rms_norm": [P, L, P, L, P, P, L, P, I, P, P, F, I, I, I, I, P],
+        "vdamd_mx_gemm": [P, L, P, L, P, P, L, P, L, I, P, P, P, I, I, I, I, I, F, F, P, I, I, P, I, I, P],
         "vdamd_layer_norm_to": [P, P, L, P, L, P, P, F, I, I, I, I, I, P],
         "vdamd_gated_rms_norm": [P, L, P, P, P, L, F, I, I, I, F, I, I, I, P],
         "vdamd_clamped_glu": [P, P, L, I, I, F, F, I, P],
@@ -2426,3 +2431,179 @@ def gated_unit_step(u, ra, ra_bias, ri, ri_bias, rate, gate, gate_bias, state, s
         return out
     a, drive = block_gates(u, ra, ra_bias, ri, ri_bias, rate)
     return gated_unit_scan(a, drive, gate, gate_bias, state, slots, query_start_loc, seq_lens, max_query_len)
+
+
+# ------------------------------------------------------------------ microscaled formats
+MX_NORM_MAX = 32768
+
+
+def _mx_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels are launched on the current device's current stream: every operand has to be there."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"operands on {device} and on {t.device}")
+    if device.index is not None and device.index != torch.cuda.current_device():
+        raise ValueError(f"operands on {device}, current device cuda:{torch.cuda.current_device()}")
+
+
+def _mx_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` as rows that the kernels can read: unit stride, 16-byte borders."""
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+        x2 = x2.contiguous()
+        if x2.data_ptr() % 16:
+            x2 = x2.clone()
+    return x2
+
+
+def mx_quantize(x: torch.Tensor, bits: int, dtype: Optional[torch.dtype] = None) -> quant.MxRows:
+    x2 = _mx_rows(x)
+    _mx_device(x.device, x2)
+    m, k = x2.shape
+    r = quant.MxRows.empty(m, k, bits, dtype or x.dtype, x.device)
+    _check(_LIB.vdamd_mx_quantize(r.payload.data_ptr(), r.payload.stride(0), r.scales.data_ptr(), r.scales.stride(0), x2.data_ptr(),
+                                  x2.stride(0), m, k, r.payload.shape[1] * 8 // bits, bits, _dt(x2), _stream()), "mx_quantize")
+    return r
+
+
+def mx_dequantize(rows: quant.MxRows, dtype: torch.dtype) -> torch.Tensor:
+    _mx_device(rows.device, rows.payload, rows.scales)
+    m, k = rows.shape
+    out = torch.empty((m, k), dtype=dtype, device=rows.device)
+    _check(_LIB.vdamd_mx_dequantize(out.data_ptr(), rows.payload.data_ptr(), rows.payload.stride(0), rows.scales.data_ptr(),
+                                    rows.scales.stride(0), m, k, rows.bits, _dt(out), _stream()), "mx_dequantize")
+    return out
+
+
+def mx_rms_norm(x: Optional[torch.Tensor], slabs: Optional[torch.Tensor], residual: Optional[torch.Tensor], weight: torch.Tensor,
+                eps: float) -> Tuple[quant.MxRows, Optional[torch.Tensor]]:
+    """``x [M, H]`` or fp32 slabs ``[ks, M, H]`` of it; returns the normed rows and the new residual (None without one)."""
+    h = weight.numel()
+    if slabs is not None:
+        assert slabs.dtype == torch.float32 and slabs.dim() == 3 and slabs.is_contiguous() and slabs.shape[2] == h
+        m, x2 = slabs.shape[1], None
+    else:
+        x2 = _mx_rows(x)
+        m = x2.shape[0]
+        assert x2.shape[1] == h and x2.dtype == weight.dtype, (x.shape, x.dtype, weight.shape, weight.dtype)
+    assert _half(weight) and weight.is_contiguous() and weight.data_ptr() % 16 == 0
+    assert h % 32 == 0 and h <= MX_NORM_MAX, f"rows of {h} values: multiples of 32 up to {MX_NORM_MAX} are normed into blocks"
+    out = None
+    if residual is not None:
+        assert residual.dtype == weight.dtype and residual.numel() == m * h and residual.shape[-1] == h
+        residual = residual.contiguous()
+        out = torch.empty_like(residual)
+    _mx_device(weight.device, x2, slabs, residual)
+    r = quant.MxRows.empty(m, h, 8, weight.dtype, weight.device)
+    _check(_LIB.vdamd_mx_rms_norm(r.payload.data_ptr(), r.payload.stride(0), r.scales.data_ptr(), r.scales.stride(0), _ptr(out),
+                                  _ptr(x2), 0 if x2 is None else x2.stride(0), _ptr(slabs), 0 if slabs is None else slabs.shape[0],
+                                  _ptr(residual), weight.data_ptr(), float(eps), m, h, r.payload.shape[1], _dt(weight), _stream()),
+           "mx_rms_norm")
+    return r, out
+
+
+def _mx_check(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor], grouped: bool) -> Tuple[int, int, int]:
+    """(matrices, rows of each, 128-column steps) of a weight that ``rows`` can be multiplied with."""
+    d = 5 if grouped else 4
+    assert rows.bits == 8 and rows.dtype in (torch.bfloat16, torch.float16), (rows.bits, rows.dtype)
+    assert w.qw.dim() == d and w.qw.dtype == torch.int32 and w.qw.is_contiguous() and tuple(w.qw.shape[-2:]) == (64, 4)
+    nt, kb = w.qw.shape[-4:-2]
+    assert w.ws.dtype == torch.uint8 and w.ws.is_contiguous() and tuple(w.ws.shape) == (*w.qw.shape[:-4], nt, (kb + 3) // 4, 64, 4)
+    assert nt == (w.rows + 15) // 16 and w.rows % 8 == 0 and w.rows > 0
+    assert rows.payload.shape[1] == 128 * kb, f"rows of {rows.width} columns, a weight of {128 * kb} with padding"
+    assert rows.payload.is_contiguous() and rows.scales.is_contiguous() and rows.scales.shape[1] >= 4 * kb
+    groups = w.qw.shape[0] if grouped else 1
+    if bias is not None:
+        assert bias.dtype == rows.dtype and bias.is_contiguous() and tuple(bias.shape) == ((groups, w.rows) if grouped else (w.rows,))
+    _mx_device(rows.device, rows.payload, rows.scales, w.qw, w.ws, bias)
+    return groups, nt, kb
+
+
+def mx_plan(m: int, n: int, kb: int) -> Tuple[int, int]:
+    """(16-row tiles a workgroup takes, K split)."""
+    mt = 1 if m <= 16 else 2 if m <= 32 else 4
+    wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
+    return mt, max(1, min((512 + wgs - 1) // wgs, kb // 8))
+
+
+def _mx_gemm(epi: int, rows: quant.MxRows, w: quant.MxWeight, bias, out, os, partial, ksplit: int, mt: int, limit: float = 0.0,
+             alpha: float = 0.0, tiles=None, src=None) -> None:
+    grouped = tiles is not None
+    groups, _, kb = _mx_check(rows, w, bias, grouped)
+    m = rows.shape[0] if src is None else src.numel()
+    _check(_LIB.vdamd_mx_gemm(_ptr(out), 0 if out is None else out.stride(0), _ptr(os), 0 if os is None else os.stride(0), _ptr(partial),
+                              rows.payload.data_ptr(), rows.payload.stride(0), rows.scales.data_ptr(), rows.scales.stride(0),
+                              rows.shape[0], w.qw.data_ptr(), w.ws.data_ptr(), _ptr(bias), m, w.rows, kb, ksplit, epi, float(limit),
+                              float(alpha), _ptr(tiles), 0 if tiles is None else tiles.shape[0], groups, _ptr(src), mt,
+                              _DT[rows.dtype], _stream()), "mx_gemm")
+
+
+def mx_linear(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _, _, kb = _mx_check(rows, w, bias, False)
+    m = rows.shape[0]
+    out = torch.empty((m, w.rows), dtype=rows.dtype, device=rows.device)
+    if m:
+        mt, ksplit = mx_plan(m, w.rows, kb)
+        partial = torch.empty((ksplit, m, w.rows), dtype=torch.float32, device=rows.device) if ksplit > 1 else None
+        _mx_gemm(0, rows, w, bias, out, None, partial, ksplit, mt)
+    return out
+
+
+def mx_linear_partials(rows: quant.MxRows, w: quant.MxWeight) -> Optional[torch.Tensor]:
+    """``mx_linear`` left as fp32 slabs ``[ks, M, N]``; None where K is not split."""
+    _, _, kb = _mx_check(rows, w, None, False)
+    m = rows.shape[0]
+    mt, ksplit = mx_plan(m, w.rows, kb) if m else (1, 1)
+    if ksplit == 1:
+        return None
+    partial = torch.empty((ksplit, m, w.rows), dtype=torch.float32, device=rows.device)
+    _mx_gemm(1, rows, w, None, None, None, partial, ksplit, mt)
+    return partial
+
+
+def _mx_gated_out(rows: quant.MxRows, w: quant.MxWeight, m: int) -> quant.MxRows:
+    assert w.rows % 256 == 0, f"{w.rows} rows of gate and up: halves of whole 128 are wanted (pack_mx with halves=2)"
+    return quant.MxRows.empty(m, w.rows // 2, 8, rows.dtype, rows.device)
+
+
+def mx_gate_up(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float, alpha: float) -> quant.MxRows:
+    m = rows.shape[0]
+    r = _mx_gated_out(rows, w, m)
+    _mx_check(rows, w, bias, False)
+    if m:
+        _mx_gemm(2, rows, w, bias, r.payload, r.scales, None, 1, mx_plan(m, w.rows, 1)[0], limit, alpha)
+    return r
+
+
+def mx_tile_rows(slots: int, experts: int) -> int:
+    """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices."""
+    avg = slots / max(1, experts)
+    return 16 if avg <= 16 else 32 if avg <= 32 else 64
+
+
+def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], device: torch.device) -> int:
+    assert tiles.dtype == torch.int32 and tiles.dim() == 2 and tiles.shape[1] == 3 and tiles.is_contiguous()
+    assert src is None or (src.dtype == torch.int32 and src.dim() == 1 and src.is_contiguous())
+    assert tile_rows in (16, 32, 64), tile_rows
+    _mx_device(device, tiles, src)
+    return tile_rows // 16
+
+
+def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor] = None,
+                      src_row: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Product of rows sorted by matrix (``moe_align``) with ``w``'s matrices; ``src_row``: the rows are ``rows[src_row]``.  Rows of no
+    tile stay unwritten."""
+    mt = _mx_tiles(tiles, tile_rows, src_row, rows.device)
+    out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=rows.dtype, device=rows.device)
+    if out.shape[0]:
+        _mx_gemm(0, rows, w, bias, out, None, None, 1, mt, tiles=tiles, src=src_row)
+    return out
+
+
+def mx_grouped_gate_up(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor],
+                       limit: float, alpha: float, src_row: Optional[torch.Tensor] = None) -> quant.MxRows:
+    mt = _mx_tiles(tiles, tile_rows, src_row, rows.device)
+    r = _mx_gated_out(rows, w, rows.shape[0] if src_row is None else src_row.numel())
+    if r.shape[0]:
+        _mx_gemm(2, rows, w, bias, r.payload, r.scales, None, 1, mt, limit, alpha, tiles, src_row)
+    return r

@@ -18,7 +18,7 @@ tensor-parallel shards have been cut.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -204,3 +204,200 @@ def quantize_fp4(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Ten
     code = (code + 8 * (blocks < 0)).to(torch.uint8).reshape(n, k // 2, 2)
     packed = code[..., 0] | (code[..., 1] << 4)
     return packed.contiguous(), bs, gscale
+
+
+# ------------------------------------------------------------------ microscaled formats (blocks of 32 values, one power of two each)
+MX_BLOCK = 32
+MX_LARGEST = {8: 448.0, 4: 6.0}      # largest element: e4m3, e2m1
+
+
+def _ceil_to(n: int, m: int) -> int:
+    return -(-n // m) * m
+
+
+class MxRows:
+    """Rows in microscaled 8- or 4-bit floating point: a value is ``element * 2^(scale byte - 127)``, one scale for each 32
+    neighbours of a row; a scale byte of 255 makes its block NaN.
+
+    ``q`` ``[M, K]`` float8_e4m3fn (8 bits) or ``[M, K/2]`` uint8 (4 bits, the even element in the low half of a byte), ``s``
+    ``[M, K/32]`` float8_e8m0fnu; ``dtype``: the type that products of these rows have.  Both are views of buffers whose rows are
+    padded (elements with zeros to a multiple of 128 columns, scales to 16 bytes), which is what the kernels read."""
+    __slots__ = ("payload", "scales", "width", "bits", "dtype")
+
+    def __init__(self, payload: torch.Tensor, scales: torch.Tensor, width: int, bits: int, dtype: torch.dtype):
+        self.payload, self.scales, self.width, self.bits, self.dtype = payload, scales, width, bits, dtype
+
+    @staticmethod
+    def empty(rows: int, width: int, bits: int, dtype: torch.dtype, device) -> "MxRows":
+        """Buffers for a kernel to fill (uninitialised)."""
+        if bits not in MX_LARGEST:
+            raise ValueError(f"microscaled rows hold 8 or 4 bits a value, not {bits}")
+        if width <= 0 or width % MX_BLOCK:
+            raise ValueError(f"{width} columns are not whole blocks of {MX_BLOCK}")
+        kp = _ceil_to(width, 128)
+        return MxRows(torch.empty((rows, kp * bits // 8), dtype=torch.uint8, device=device),
+                      torch.empty((rows, _ceil_to(kp // MX_BLOCK, 16)), dtype=torch.uint8, device=device), width, bits, dtype)
+
+    @staticmethod
+    def of(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> "MxRows":
+        """Rows from elements and scales that come from elsewhere (``q`` and ``s`` as the properties have them, ``s`` also uint8)."""
+        bits = 8 if q.dtype == torch.float8_e4m3fn else 4
+        if q.dtype not in (torch.float8_e4m3fn, torch.uint8) or s.dtype not in (torch.float8_e8m0fnu, torch.uint8):
+            raise TypeError(f"microscaled rows of {q.dtype} elements and {s.dtype} scales")
+        width = q.shape[-1] * (8 // bits)
+        if q.dim() != 2 or s.dim() != 2 or width % MX_BLOCK or tuple(s.shape) != (q.shape[0], width // MX_BLOCK):
+            raise ValueError(f"elements {tuple(q.shape)} and scales {tuple(s.shape)} are not rows of blocks of {MX_BLOCK}")
+        r = MxRows.empty(q.shape[0], width, bits, dtype, q.device)
+        r.payload.zero_()
+        r.payload[:, :q.shape[1]] = q.view(torch.uint8)
+        r.scales[:, :s.shape[1]] = s.view(torch.uint8)
+        return r
+
+    @property
+    def q(self) -> torch.Tensor:
+        p = self.payload[:, :self.width * self.bits // 8]
+        return p.view(torch.float8_e4m3fn) if self.bits == 8 else p
+
+    @property
+    def s(self) -> torch.Tensor:
+        return self.scales[:, :self.width // MX_BLOCK].view(torch.float8_e8m0fnu)
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.payload.shape[0], self.width)
+
+    @property
+    def device(self) -> torch.device:
+        return self.payload.device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.payload.is_cuda
+
+
+class MxWeight(NamedTuple):
+    """A 4-bit microscaled weight (or several of one shape) in the kernels' layout, and its number of rows without padding.
+
+    ``qw [.., N/16, K/128, 64, 4] int32``: tiles as ``pack_fp4`` lays them out; ``ws [.., N/16, K/512, 64, 4] uint8``: byte ``i``
+    of lane ``c + 16 g`` is the scale of row ``c`` of the tile, block ``16 j + 4 i + g`` of its columns.  Rows are padded with zeros
+    to a multiple of 16, columns to 128 (of ``ws`` to 512)."""
+    qw: torch.Tensor
+    ws: torch.Tensor
+    rows: int
+
+
+def pack_mx(packed: torch.Tensor, scales: torch.Tensor, halves: int = 1) -> MxWeight:
+    """4-bit blocks in the order checkpoints have them (``packed [.., N, K/2] uint8``, the even element in the low half;
+    ``scales [.., N, K/32]`` biased exponents, uint8 or float8_e8m0fnu) -> ``MxWeight``.  ``halves`` 2: the rows are
+    ``[gate ; up]``, each padded to a multiple of 128 (the columns of the projection that follows come in whole steps)."""
+    lead, n, k = packed.shape[:-2], packed.shape[-2], packed.shape[-1] * 2
+    if packed.dtype != torch.uint8 or k % MX_BLOCK or tuple(scales.shape) != (*lead, n, k // MX_BLOCK):
+        raise ValueError(f"codes {tuple(packed.shape)} {packed.dtype} and scales {tuple(scales.shape)} are not 4-bit blocks of {MX_BLOCK}")
+    if halves not in (1, 2) or n % halves or n % (8 * halves):
+        raise ValueError(f"{n} rows in {halves} part(s): multiples of 8 are wanted")
+    sb = scales.view(torch.uint8)
+    np_ = _ceil_to(n // halves, 128 if halves == 2 else 16) * halves
+    kp, ks = _ceil_to(k, 128), _ceil_to(k, 512)
+    pad_rows = (np_ - n) // halves
+
+    def padded(t: torch.Tensor, cols: int) -> torch.Tensor:
+        t = t.reshape(*lead, halves, n // halves, t.shape[-1])
+        t = torch.nn.functional.pad(t, (0, cols - t.shape[-1], 0, pad_rows))
+        return t.reshape(*lead, np_, cols)
+    nl = len(lead)
+    order = list(range(nl))
+    words = padded(packed, kp // 2).contiguous().view(torch.int32).reshape(*lead, np_ // 16, 16, kp // 128, 4, 4)      # nt c kb g w
+    qw = words.permute(*order, nl, nl + 2, nl + 3, nl + 1, nl + 4).reshape(*lead, np_ // 16, kp // 128, 64, 4).contiguous()
+    sc = padded(sb, ks // MX_BLOCK).reshape(*lead, np_ // 16, 16, ks // 512, 4, 4)                                     # nt c j i g
+    ws = sc.permute(*order, nl, nl + 2, nl + 4, nl + 1, nl + 3).reshape(*lead, np_ // 16, ks // 512, 64, 4).contiguous()
+    return MxWeight(qw, ws, np_ if halves == 2 else n)
+
+
+def pad_mx_bias(bias: torch.Tensor, halves: int = 1) -> torch.Tensor:
+    """``bias [.., N]`` for the padded rows of ``pack_mx``."""
+    n = bias.shape[-1] // halves
+    np_ = _ceil_to(n, 128) if halves == 2 else n
+    b = bias.reshape(*bias.shape[:-1], halves, n)
+    return torch.nn.functional.pad(b, (0, np_ - n)).reshape(*bias.shape[:-1], halves * np_).contiguous()
+
+
+def unpack_mx(w: MxWeight) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Inverse of ``pack_mx`` up to the padding: ``(packed [.., N, Kp/2], scales [.., N, Kp/32])``."""
+    lead, (nt, kb), nj = w.qw.shape[:-4], w.qw.shape[-4:-2], w.ws.shape[-3]
+    nl = len(lead)
+    order = list(range(nl))
+    q = w.qw.reshape(*lead, nt, kb, 4, 16, 4).permute(*order, nl, nl + 3, nl + 1, nl + 2, nl + 4).contiguous()     # nt c kb g w
+    q = q.view(torch.uint8).reshape(*lead, nt * 16, kb * 64)[..., :w.rows, :]
+    s = w.ws.reshape(*lead, nt, nj, 4, 16, 4).permute(*order, nl, nl + 3, nl + 1, nl + 4, nl + 2)                  # nt c j i g
+    return q, s.reshape(*lead, nt * 16, nj * 16)[..., :w.rows, :kb * 4]
+
+
+def mx_blocks(x: torch.Tensor, bits: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``x [.., K]`` -> (elements as numbers ``[.., K/32, 32]``, scale bytes ``[.., K/32]``), in 32 bits: the definition."""
+    b = x.to(torch.float32).reshape(*x.shape[:-1], x.shape[-1] // MX_BLOCK, MX_BLOCK)
+    a = b.abs().amax(-1, keepdim=True)
+    finite = torch.isfinite(b).all(-1, keepdim=True)
+    a = torch.where(finite, a, torch.zeros_like(a))
+    m, e = torch.frexp(a)
+    # the smallest e with a <= largest * 2^e; 448 = 0.875 * 2^9, 6 = 0.75 * 2^3
+    e = e - (9 if bits == 8 else 3) + (m > (0.875 if bits == 8 else 0.75)).to(e.dtype)
+    e = torch.where(a > 0, e, torch.full_like(e, -127)).clamp(-127, 127)
+    u = torch.ldexp(torch.where(finite, b, torch.zeros_like(b)), -e)
+    if bits == 8:
+        u = u.to(torch.float8_e4m3fn).to(torch.float32)
+    else:
+        t = u.abs()
+        step = torch.where(t < 2, 0.5, torch.where(t < 4, 1.0, 2.0))
+        u = torch.copysign(torch.round(t / step) * step, u)
+    byte = torch.where(finite, e + 127, torch.full_like(e, 255))
+    return u, byte.squeeze(-1).to(torch.uint8)
+
+
+def mx_quantize(x: torch.Tensor, bits: int, dtype: Optional[torch.dtype] = None) -> MxRows:
+    """Reference path of ``ops.mx_quantize``."""
+    u, byte = mx_blocks(x, bits)
+    if bits == 8:
+        q = u.reshape(x.shape).to(torch.float8_e4m3fn)
+    else:
+        code = torch.tensor([0, 1, 2, 3, 4, 0, 5, 0, 6, 0, 0, 0, 7], dtype=torch.uint8, device=x.device)[(u.abs() * 2).long()]
+        code = (code | (torch.signbit(u).to(torch.uint8) << 3)).reshape(*x.shape[:-1], x.shape[-1] // 2, 2)
+        q = code[..., 0] | (code[..., 1] << 4)
+    return MxRows.of(q, byte, dtype or x.dtype)
+
+
+def _mx_scaled(u: torch.Tensor, byte: torch.Tensor) -> torch.Tensor:
+    e = byte.to(torch.int32) - 127
+    v = torch.ldexp(u.to(torch.float32), e.unsqueeze(-1))
+    return torch.where((byte == 255).unsqueeze(-1), torch.full_like(v, float("nan")), v)
+
+
+def mx_dequantize(rows: MxRows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Reference path of ``ops.mx_dequantize``."""
+    s = rows.s.view(torch.uint8)
+    if rows.bits == 8:
+        u = rows.q.to(torch.float32)
+    else:
+        u = fp4_lut(rows.device)[torch.stack([rows.q & 15, rows.q >> 4], dim=-1).long()]
+    return _mx_scaled(u.reshape(*s.shape, MX_BLOCK), s).reshape(rows.shape).to(dtype)
+
+
+def mx_weight_dense(w: MxWeight) -> torch.Tensor:
+    """The weight as fp32 ``[.., N, Kp]`` (columns from K on are zeros)."""
+    q, s = unpack_mx(w)
+    u = fp4_lut(q.device)[torch.stack([q & 15, q >> 4], dim=-1).long()]
+    return _mx_scaled(u.reshape(*s.shape, MX_BLOCK), s).reshape(*q.shape[:-1], -1)
+
+
+def mx_product(rows: MxRows, w: MxWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Reference product in fp32."""
+    y = mx_dequantize(rows) @ mx_weight_dense(w)[:, :rows.width].t()
+    return y if bias is None else y + bias.to(torch.float32)
+
+
+def mx_gated(h: torch.Tensor, limit: float, alpha: float) -> torch.Tensor:
+    """The gated activation of ``h = [gate | up]``: SiLU(gate) * up, or with a limit the clamped form of gpt-oss."""
+    g, u = h.chunk(2, dim=-1)
+    if limit > 0:
+        g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+        return (u + 1) * g * torch.sigmoid(alpha * g)
+    return g * torch.sigmoid(g) * u

@@ -1174,3 +1174,33 @@ def gated_unit_step(u: torch.Tensor, ra: torch.Tensor, ra_bias: torch.Tensor, ri
     """``block_gates`` and ``gated_unit_scan`` one after the other."""
     a, drive = block_gates(u, ra, ra_bias, ri, ri_bias, rate)
     return gated_unit_scan(a, drive, gate, gate_bias, state, slots, query_start_loc, seq_lens)
+
+
+# ------------------------------------------------------------------ microscaled formats
+def rms_norm_mx(x, residual, weight, eps):
+    """``(8-bit microscaled rows of the norm, new residual)`` in 32 bits; the norm is taken of the unrounded sum."""
+    from . import quant
+    v, out = x.float(), None
+    if residual is not None:
+        v = v + residual.float()
+        out = v.to(residual.dtype)
+    v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * weight.float()
+    return quant.mx_quantize(v.reshape(-1, v.shape[-1]), 8, weight.dtype), out
+
+
+def mx_experts(rows, topw, topi, weight13, weight2, bias13, bias2, expert_start: int, limit: float, alpha: float):
+    from . import quant
+    x = quant.mx_dequantize(rows)
+    out = torch.zeros(x.shape[0], weight2.rows, dtype=torch.float32, device=x.device)
+    for e in range(weight13.qw.shape[0]):
+        t, j = (topi == e + expert_start).nonzero(as_tuple=True)
+        if not t.numel():
+            continue
+        w13 = quant.MxWeight(weight13.qw[e], weight13.ws[e], weight13.rows)
+        w2 = quant.MxWeight(weight2.qw[e], weight2.ws[e], weight2.rows)
+        h = x[t] @ quant.mx_weight_dense(w13)[:, :x.shape[1]].t()
+        h = h if bias13 is None else h + bias13[e].float()
+        a = quant.mx_quantize(quant.mx_gated(h, limit, alpha), 8, rows.dtype)
+        y = quant.mx_product(a, w2, None if bias2 is None else bias2[e])
+        out.index_add_(0, t, y.to(rows.dtype).float() * topw[t, j].float().unsqueeze(1))
+    return out.to(rows.dtype)
