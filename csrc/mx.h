@@ -10,6 +10,7 @@
 
 typedef uint32_t mx_u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t mx_u32x4 __attribute__((ext_vector_type(4)));
+typedef int mx_i32x4 __attribute__((ext_vector_type(4)));
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
 
 // the scale byte of a block whose largest |v| is `amax` (448 = 1.75 * 2^8, 6 = 1.5 * 2^2).  `amax` as its bits: of non-negative

@@ -31,13 +31,18 @@ struct MxArgs {
   const int* tiles; int num_tiles; int groups; const int* src; int x_rows;
 };
 
-__device__ __forceinline__ f32x4 mx_mfma(mx_u32x4 w, mx_u32x4 x0, mx_u32x4 x1, f32x4 c, uint32_t sw, uint32_t sx) {
+__device__ __forceinline__ f32x4 mx_mfma(mx_u32x4 w, mx_i32x8 x, f32x4 c, uint32_t sw, uint32_t sx) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const mx_i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-  const mx_i32x8 b = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
-  c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, (int)sw, 0, (int)sx);
+  const mx_i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};      // (the 4-bit form reads four registers)
+  c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, c, 4, 0, 0, (int)sw, 0, (int)sx);
 #endif
   return c;
+}
+
+// the two 16-byte halves of an 8-bit fragment
+template <typename P> __device__ __forceinline__ mx_i32x8 mx_fragment(const P* lo, const P* hi) {
+  const mx_i32x4 a = *reinterpret_cast<const mx_i32x4*>(lo), b = *reinterpret_cast<const mx_i32x4*>(hi);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 __device__ __forceinline__ float mx_glu(float g, float u, float limit, float alpha) {
@@ -49,22 +54,29 @@ __device__ __forceinline__ float mx_glu(float g, float u, float limit, float alp
   return g * fast_sigmoid(g) * u;
 }
 
-// 16 gated values of a row's block of 32 are with each of four lanes (r, q), 4 columns from 4 q of both 16-column halves: elements and scale
+// A row's block of 32 gated values is with four lanes (r, q), 4 columns from 4 q of both its 16-column halves: elements and scale.  All
+// 64 lanes run; ok: the row is stored
 __device__ __forceinline__ void mx_store_block(uint8_t* q, uint8_t* s, const float (&a)[2][4], int lane, bool ok) {
+#if defined(__HIP_DEVICE_COMPILE__)
   uint32_t m = 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int r = 0; r < 4; ++r) m = max(m, mx_abs_bits(a[h][r]));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+  const auto far = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = max((uint32_t)far[0], (uint32_t)far[1]);
+  const auto near = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = max((uint32_t)near[0], (uint32_t)near[1]);
   const uint32_t byte = mx_scale_byte<8>(m);
   const float inv = mx_inverse(byte);
+  // lanes of even q trade their second half for the first of the lane after them: eight neighbouring bytes each
+  const auto w = __builtin_amdgcn_permlane16_swap(mx_pack_fp8(a[0][0], a[0][1], a[0][2], a[0][3], inv),
+                                                  mx_pack_fp8(a[1][0], a[1][1], a[1][2], a[1][3], inv), false, false);
+  const int at = lane >> 4;
   if (!ok) return;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    *reinterpret_cast<uint32_t*>(q + 16 * h + 4 * (lane >> 4)) = mx_pack_fp8(a[h][0], a[h][1], a[h][2], a[h][3], inv);
+  *reinterpret_cast<mx_u32x2*>(q + ((at & 1) ? 16 + 4 * (at - 1) : 4 * at)) = mx_u32x2{(uint32_t)w[0], (uint32_t)w[1]};
   if (lane < 16) *s = (uint8_t)byte;
+#endif
 }
 
 // Few rows: the weights' bytes are the time.  A workgroup has four 16-column tiles (MX_GLU: two of the gate and the two of the same
@@ -114,7 +126,8 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  mx_u32x4 w[2][MX_NT], x0[2][MT], x1[2][MT];
+  mx_u32x4 w[2][MX_NT];
+  mx_i32x8 x[2][MT];
   uint32_t sw[2][MX_NT], sx[2][MT];
   auto load = [&](int b, int k) {
 #pragma unroll
@@ -124,8 +137,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      x0[b][i] = *reinterpret_cast<const mx_u32x4*>(xp[i] + 128L * k);
-      x1[b][i] = *reinterpret_cast<const mx_u32x4*>(xp[i] + 128L * k + 64);
+      x[b][i] = mx_fragment(xp[i] + 128L * k, xp[i] + 128L * k + 64);
       sx[b][i] = sp[i][4 * k];
     }
   };
@@ -133,7 +145,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
 #pragma unroll
     for (int t = 0; t < MX_NT; ++t)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[t][i] = mx_mfma(w[b][t], x0[b][i], x1[b][i], acc[t][i], sw[b][t], sx[b][i]);
+      for (int i = 0; i < MT; ++i) acc[t][i] = mx_mfma(w[b][t], x[b][i], acc[t][i], sw[b][t], sx[b][i]);
   };
   if (lo < hi) load(0, lo);
   for (int k = lo; k < hi; k += 2) {
@@ -188,6 +200,295 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
   }
 }
 
+// Many rows: the matrix cores are the time.  256 x 256 outputs a tile (MX_GLU: 128 columns of the gate and the same of the up half), one
+// persistent workgroup of eight waves a compute unit, K in steps of 128.
+//  * Both operands go from memory to LDS without passing through registers.  A step is four images: A0, A1 (128 rows x 128 bytes of
+//    x; the 16-byte slots of a row XOR-ed with (row >> 1) & 7 at the source, so that the lanes of a fragment read meet no bank twice)
+//    and B0, B1 (eight weight tiles of 1 KiB, in the order in which lanes read them).  Two sets of images.
+//  * A wave has 128 x 64 outputs as four quadrants of 64 x 32, quadrant (mq, nq) from images A<mq> and B<nq>; a step is four phases of
+//    eight matrix instructions, one quadrant each, every fragment read once: A0 in phase 0, A1 in 1, B1 in 2, the next step's B0 in 3.
+//  * The loads are one stream that never drains: image h = 4 t + (A0, B0, A1, B1) is issued in phase h - 6, and a phase waits until all
+//    but the newest four images (three in phase 2, ahead of the early read) are there: 6 and 5 loads, an A image being two loads of a
+//    wave and a B image one.  It runs on through the output tiles.
+//  * Scales come 16 bytes a row (four steps) at a time into two further sets, one load of each wave in every other step, at its third
+//    phase: one more in the counts from there to its sixth.  Lanes read their byte from LDS.
+//  * Waves 4-7 run one barrier behind waves 0-3: on each SIMD one wave multiplies while the other reads.
+//  * An odd number of steps gets one more, whose weights are zeros: loads out of the descriptor's range.
+constexpr int MXB_A = 128 * 128, MXB_B = 8 * 1024, MXB_SET = 2 * MXB_A + 2 * MXB_B, MXB_SC = 2 * 4096;
+typedef __attribute__((address_space(3))) void mx_lds_void;
+
+template <typename T, int EPI, bool grouped>
+__global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, int ntn) {
+#if defined(__HIP_DEVICE_COMPILE__)      // the buffer-descriptor builtins exist in the device pass only
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * MXB_SET + 2 * MXB_SC];
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wid >> 2, wc = wid & 3;
+  const int r16 = lane & 15, q = lane >> 4;
+  const int KB = a.KB, SS = (KB + 3) >> 2, KT = (KB + 1) & ~1, ntiles = (a.N + 15) >> 4;
+
+  // ---- this workgroup's tiles: bands of 8 row tiles, in a band every XCD a range of tile columns, column by column (as the 16-bit
+  // product's large tiles: 32 workgroups of an XCD share 12 panels in its L2).  Grouped: units of two row tiles and all columns of an
+  // eighth, dealt to the XCDs in turn
+  const int xcd = blockIdx.x & 7, stride = gridDim.x >> 3;
+  const int c0 = (int)((long)ntn * xcd >> 3), c1 = (int)((long)ntn * (xcd + 1) >> 3), ncols = c1 - c0;
+  const int gparts = ntn >= 16 ? ntn / 8 : 1, gcols = (ntn + gparts - 1) / gparts;
+  const int units = ((ntm + 1) / 2 * gparts - xcd + 7) / 8;
+  const int chunk_end = grouped ? units * 2 * gcols : ntm * ncols;
+  auto unit_of = [&](int tl) { return xcd + 8 * (tl / (2 * gcols)); };
+  auto row_tile = [&](int tl) { return 2 * (unit_of(tl) / gparts) + (tl & 1); };
+  auto column = [&](int tl) { return unit_of(tl) % gparts * gcols + (tl % (2 * gcols) >> 1); };
+  auto entry = [&](int rt, int i) { return __builtin_amdgcn_readfirstlane(a.tiles[3 * rt + i]); };
+  auto used = [&](int tl) {                  // the first entry with rows from tl on
+    if (grouped)
+      while (tl < chunk_end) {
+        const int rt = row_tile(tl);
+        if (rt < ntm && column(tl) < ntn && entry(rt, 2) > 0) break;
+        tl += stride;
+      }
+    return tl;
+  };
+  int tile = used(blockIdx.x >> 3);
+  if (tile >= chunk_end) return;
+  auto decode = [&](int tl, int& m0, int& end, int& tn, int& g) {      // first row, row limit, tile column, matrix
+    if (grouped) {
+      const int rt = row_tile(tl);
+      g = min(max(entry(rt, 0), 0), a.groups - 1);
+      m0 = min(max(entry(rt, 1), 0), a.M - 1);
+      end = min(a.M, m0 + min(entry(rt, 2), 256));
+      tn = column(tl);
+      return;
+    }
+    const int band = tl / (8 * ncols), rows = min(8, ntm - 8 * band), in = tl - band * 8 * ncols;
+    m0 = (8 * band + in % rows) * 256;
+    end = a.M;
+    tn = c0 + in / rows;
+    g = 0;
+  };
+
+  // ---- staging.  Everything that depends on the output tile is scalar; rows and weight tiles past the end are out of their
+  // descriptors' range and come as zeros
+  const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.xq), 0, (int)(unsigned)((long)a.x_rows * a.ldq), 0x00020000);
+  const unsigned wbytes = (unsigned)((long)ntiles * KB * 1024), sbytes = (unsigned)((long)ntiles * SS * 256);
+  const unsigned ldq = (unsigned)a.ldq, half_tiles = ntiles >> 1;
+  struct Stage { unsigned rows, b0, b1, sc; int g; };        // byte offsets of the tile's rows, weight tiles and scales of this wave
+  auto stage_of = [&](int tl) {
+    int m0, end, tn, g;
+    decode(tl, m0, end, tn, g);
+    const unsigned t0 = EPI == MX_GLU ? 8 * tn : 16 * tn, t1 = EPI == MX_GLU ? half_tiles + 8 * tn : 16 * tn + 8;
+    const unsigned i = 4 * (wid & 1);
+    return Stage{(unsigned)(m0 + 16 * wid) * ldq, (t0 + wid) * (unsigned)(KB * 1024), (t1 + wid) * (unsigned)(KB * 1024),
+                 wid < 4 ? (unsigned)(m0 + 64 * wid) * (unsigned)a.lds : ((wid < 6 ? t0 : t1) + i) * (unsigned)(SS * 256), g};
+  };
+  auto weights = [&](int g) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.qw + (long)g * wbytes), 0, (int)wbytes, 0x00020000);
+  };
+  auto scales = [&](int g) {
+    return wid < 4 ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.xs), 0, (int)(unsigned)((long)a.x_rows * a.lds), 0x00020000)
+                   : __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.ws + (long)g * sbytes), 0, (int)sbytes, 0x00020000);
+  };
+  const unsigned lane_a = (unsigned)(lane >> 3) * ldq + 16 * ((lane & 7) ^ (lane >> 4)), lane_b = 16 * lane;
+  const unsigned lane_s = wid < 4 ? (unsigned)lane * (unsigned)a.lds : (unsigned)(lane >> 4) * (unsigned)(SS * 256) + 16 * (lane & 15);
+  auto wrs = weights(0);
+  auto srs = scales(0);
+  Stage cur, nxt;                            // of the tile being staged, of the one after it
+  // steps past the last address the staging tile's first: by then `cur` is the next output tile's.  The step of zeros takes x from the
+  // last one
+  auto stage_a = [&](int half, int set, int kt) {
+    const int k = min(kt >= KT ? kt - KT : kt, KB - 1);
+    const unsigned off = lane_a + (cur.rows + (unsigned)half * 128 * ldq);
+    unsigned char* const to = smem + set * MXB_SET + half * MXB_A + 2048 * wid;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mx_lds_void*)to, 16, off, k * 128, 0, 0);
+    // (eight rows on: the slots' XOR differs by 4; ldq is a multiple of 128)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mx_lds_void*)(to + 1024), 16, (off + 8 * ldq) ^ 64, k * 128, 0, 0);
+  };
+  auto stage_b = [&](int half, int set, int kt) {
+    const int k = kt >= KT ? kt - KT : kt;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (mx_lds_void*)(smem + set * MXB_SET + 2 * MXB_A + half * MXB_B + wid * 1024), 16,
+                                             k < KB ? lane_b + (half ? cur.b1 : cur.b0) : 0xfffffff0u, k < KB ? k * 1024 : 0, 0, 0);
+  };
+  auto stage_s = [&](int set, int ss) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(srs, (mx_lds_void*)(smem + 2 * MXB_SET + set * MXB_SC + wid * 1024), 16, lane_s + cur.sc,
+                                             ss * (wid < 4 ? 16 : 256), 0, 0);
+  };
+
+  // ---- fragments
+  const int swz = (r16 >> 1) & 7, so0 = (q ^ swz) << 4, so1 = ((4 + q) ^ swz) << 4;
+  const int xro = (wr * 64 + r16) * 128, wro = 2 * MXB_A + wc * 2048 + lane * 16;
+  const int xso = 2 * MXB_SET + (wr * 64 + r16) * 16 + q, wso = 2 * MXB_SET + 4096 + wc * 512 + lane * 4;
+  auto read_x = [&](mx_i32x8 (&f)[4], uint32_t (&s)[4], int set, int half, int sbyte) {
+    const unsigned char* b = smem + set * MXB_SET + half * MXB_A + xro;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = mx_fragment(b + i * 2048 + so0, b + i * 2048 + so1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = smem[xso + sbyte + half * 2048 + i * 256];
+  };
+  auto read_w = [&](mx_u32x4 (&f)[2], uint32_t (&s)[2], int set, int half, int sbyte, int step) {
+    const unsigned char* b = smem + set * MXB_SET + half * MXB_B + wro;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) f[j] = *reinterpret_cast<const mx_u32x4*>(b + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = smem[wso + sbyte + step + half * 2048 + j * 256];
+  };
+  f32x4 acc00[4][2], acc10[4][2], acc11[4][2], acc01[4][2];
+  auto mma = [&](f32x4 (&acc)[4][2], const mx_i32x8 (&xf)[4], const uint32_t (&sx)[4], const mx_u32x4 (&wf)[2], const uint32_t (&sw)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mx_mfma(wf[j], xf[i], acc[i][j], sw[j], sx[i]);
+  };
+  mx_i32x8 xf0[4], xf1[4];
+  mx_u32x4 wf0[2], wf1[2];
+  uint32_t sx0[4], sx1[4], sw0[2], sw1[2];
+
+#define MXB_PHASE(READS, STAGE, WAITN, ACC, XF, SX, WF, SW)                            \
+  READS;                                                                               \
+  STAGE;                                                                               \
+  __builtin_amdgcn_sched_barrier(0);                                                   \
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WAITN) : "memory");                         \
+  __builtin_amdgcn_s_barrier();                                                        \
+  __builtin_amdgcn_sched_barrier(0);                                                   \
+  __builtin_amdgcn_s_setprio(1);                                                       \
+  mma(ACC, XF, SX, WF, SW);                                                            \
+  __builtin_amdgcn_s_setprio(0);                                                       \
+  __builtin_amdgcn_sched_barrier(0);                                                   \
+  __builtin_amdgcn_s_barrier();                                                        \
+  __builtin_amdgcn_sched_barrier(0);
+
+  int cm0, cend, ctn, cg;                    // the tile being computed (the staging tile runs ahead)
+  decode(tile, cm0, cend, ctn, cg);
+  cur = stage_of(tile);
+  wrs = weights(cur.g);
+  srs = scales(cur.g);
+  int par = 0;                               // which set holds the scales of the current four steps
+  stage_s(0, 0);
+  stage_a(0, 0, 0); stage_b(0, 0, 0); stage_a(1, 0, 0); stage_b(1, 0, 0);
+  stage_a(0, 1, 1); stage_b(0, 1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  if (wr == 1) __builtin_amdgcn_s_barrier();          // waves 4-7 run one barrier behind
+  __builtin_amdgcn_sched_barrier(0);
+  read_w(wf0, sw0, 0, 0, 0, 0);
+
+  for (;;) {
+    const int next = used(tile + stride);
+    const bool has_next = next < chunk_end;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc00[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        acc10[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        acc11[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        acc01[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    nxt = stage_of(has_next ? next : tile);
+    // One body without a branch: the compiler would move a phase's products behind it, past their barriers.  In the last two steps
+    // everything staged from the third phase on is the next output tile's.  Scales are loaded in every other step, so twice each; the
+    // first time into a set that is free already.
+    for (int t = 0; t < KT; t += 2) {
+      const int s0 = min(t, KB - 1) & 3, s1 = min(t + 1, KB - 1) & 3;      // (the step of zeros takes its neighbour's scales)
+      const bool last = t == KT - 2;
+      const int now = par * MXB_SC;
+      MXB_PHASE(read_x(xf0, sx0, 0, 0, now + 4 * s0), stage_a(1, 1, t + 1), 6, acc00, xf0, sx0, wf0, sw0)
+      MXB_PHASE(read_x(xf1, sx1, 0, 1, now + 4 * s0), stage_b(1, 1, t + 1), 6, acc10, xf1, sx1, wf0, sw0)
+      cur.rows = last ? nxt.rows : cur.rows;
+      cur.b0 = last ? nxt.b0 : cur.b0;
+      cur.b1 = last ? nxt.b1 : cur.b1;
+      cur.sc = last ? nxt.sc : cur.sc;
+      if constexpr (grouped) {
+        cur.g = last ? nxt.g : cur.g;
+        wrs = weights(cur.g);
+        srs = scales(cur.g);
+      }
+      MXB_PHASE(read_w(wf1, sw1, 0, 1, now, s0), stage_s(par ^ 1, last ? 0 : (t >> 2) + 1); stage_a(0, 0, t + 2), 6, acc11, xf1, sx1, wf1, sw1)
+      MXB_PHASE(read_w(wf0, sw0, 1, 0, now, s1), stage_b(0, 0, t + 2), 7, acc01, xf0, sx0, wf1, sw1)
+      MXB_PHASE(read_x(xf0, sx0, 1, 0, now + 4 * s1), stage_a(1, 0, t + 2), 7, acc00, xf0, sx0, wf0, sw0)
+      MXB_PHASE(read_x(xf1, sx1, 1, 1, now + 4 * s1), stage_b(1, 0, t + 2), 7, acc10, xf1, sx1, wf0, sw0)
+      par ^= (int)(last || (t & 2));
+      MXB_PHASE(read_w(wf1, sw1, 1, 1, now, s1), stage_a(0, 1, t + 3), 5, acc11, xf1, sx1, wf1, sw1)
+      MXB_PHASE(read_w(wf0, sw0, 0, 0, par * MXB_SC, last ? 0 : (t + 2) & 3), stage_b(0, 1, t + 3), 6, acc01, xf0, sx0, wf1, sw1)
+    }
+    // nothing below may be computed before the K loop (it would be live across it)
+    asm volatile("" : "+s"(cm0), "+s"(ctn), "+s"(cend), "+s"(cg));
+
+    // ---- lane (r16, q) of fragment (i, j) holds columns 16 j + 4 q .. + 3 of row 16 i + r16 of its quadrant
+    int eln = lane;
+    asm volatile("" : "+v"(eln));
+    const int er = eln & 15, eq = eln >> 4;
+    auto put = [&](const f32x4 (&a0)[4][2], const f32x4 (&a1)[4][2], int mq) {
+      const T* bias = a.bias == nullptr ? nullptr : (const T*)a.bias + (long)cg * a.N;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = cm0 + 128 * mq + 64 * wr + 16 * i + er;
+        if constexpr (EPI == MX_GLU) {
+          const int half = a.N >> 1, n = 128 * ctn + 32 * wc;
+          float v[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int c = n + 16 * j + 4 * eq + e;
+              v[j][e] = mx_glu(a0[i][j][e] + (bias ? (float)bias[c] : 0.f), a1[i][j][e] + (bias ? (float)bias[half + c] : 0.f),
+                               a.limit, a.alpha);
+            }
+          mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n, a.os + (long)m * a.ldos + (n >> 5), v, eln, m < cend);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int n = 256 * ctn + 128 * h + 32 * wc + 16 * j + 4 * eq;
+              const f32x4 v = h ? a1[i][j] : a0[i][j];
+              if (m < cend && n < a.N) {
+                typename Vec4<T>::type o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (T)(v[e] + (bias ? (float)bias[n + e] : 0.f));
+                *reinterpret_cast<typename Vec4<T>::type*>((T*)a.out + (long)m * a.ldo + n) = o;
+              }
+            }
+        }
+      }
+    };
+    put(acc00, acc01, 0);
+    put(acc10, acc11, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!has_next) break;
+    tile = next;
+    decode(tile, cm0, cend, ctn, cg);
+  }
+#undef MXB_PHASE
+  if (wr == 0) __builtin_amdgcn_s_barrier();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the tail's loads must not outlive the LDS
+#endif
+}
+
+int mx_num_cus() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 8) return 256;
+  return n;
+}
+
+// (row_tiles == 16)
+template <typename T, int EPI>
+int mx_big(const MxArgs& a, hipStream_t st) {
+  const long lim = (1L << 32) - 64;
+  if ((long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim) return -8;
+  const int ntn = EPI == MX_GLU ? (a.N / 2 + 127) / 128 : (a.N + 255) / 256;
+  const int ntm = a.tiles != nullptr ? a.num_tiles : (a.M + 255) / 256;
+  const int gparts = ntn >= 16 ? ntn / 8 : 1;
+  const long per = a.tiles != nullptr ? ((ntm + 1L) / 2 * gparts + 7) / 8 * 2 * ((ntn + gparts - 1) / gparts) : (long)ntm * ((ntn + 7) / 8);
+  if (per >= (1L << 30)) return -7;
+  const int cus = mx_num_cus() / 8;
+  const unsigned grid = 8 * (unsigned)(per < cus ? per : cus);
+  if (a.tiles != nullptr) mx_big_kernel<T, EPI, true><<<grid, 512, 0, st>>>(a, ntm, ntn);
+  else mx_big_kernel<T, EPI, false><<<grid, 512, 0, st>>>(a, ntm, ntn);
+  HIP_LAUNCH_CHECK();
+  return 0;
+}
+
 // y = sum of the slabs + bias
 template <typename T>
 __global__ __launch_bounds__(256) void mx_reduce_kernel(T* __restrict__ out, long ldo, const float* __restrict__ partial,
@@ -221,6 +522,10 @@ int mx_stream(const MxArgs& a, int mt, hipStream_t st) {
 
 template <typename T>
 int mx_dispatch(const MxArgs& a, int epi, int mt, hipStream_t st) {
+  if (mt == 16) {
+    if (a.ksplit != 1 || a.src != nullptr) return -1;
+    return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : -1;
+  }
   if (epi == MX_GLU) return mx_stream<T, MX_GLU>(a, mt, st);
   if (epi == MX_SLAB || a.ksplit > 1) {
     const int rc = mx_stream<T, MX_SLAB>(a, mt, st);
@@ -235,19 +540,20 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, hipStream_t st) {
 
 }  // namespace
 
-// xq [x_rows][128 KB] bytes (rows ldq apart, a multiple of 16), xs [x_rows][4 KB] scale bytes (rows lds apart, a multiple of 4); qw, ws as
+// xq [x_rows][128 KB] bytes (rows ldq apart, a multiple of 128), xs [x_rows][4 KB] scale bytes (rows lds apart, a multiple of 4); qw, ws as
 // above for `groups` matrices of N rows (padded to 16), N % 8 == 0.
 // epi 0: out [M][N] of the model type, rows ldo elements apart (ksplit > 1: through partial [ksplit][M][N]); 1: partial alone;
 // 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales, ksplit 1; limit 0: SiLU.
 // tiles [num_tiles][3] (matrix, first row, rows) or null; src [M] or null: the row of x behind each row.  row_tiles: 16-row tiles a
-// workgroup takes (1, 2 or 4; of `tiles` at most 16 row_tiles rows each).
+// workgroup takes (1, 2 or 4; of `tiles` at most 16 row_tiles rows each); 16: the kernel of 256-row tiles (ksplit 1, src null, x_rows ldq
+// and a matrix's bytes below 2^32, lds a multiple of 16).
 VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* partial, const void* xq, long ldq, const void* xs, long lds,
                             int x_rows, const void* qw, const void* ws, const void* bias, int M, int N, int KB, int ksplit, int epi,
                             float limit, float alpha, const int* tiles, int num_tiles, int groups, const int* src, int row_tiles,
                             int dtype, void* stream) {
   if (M <= 0 || (tiles != nullptr && num_tiles <= 0)) return 0;
   if (N <= 0 || N % 8 || KB <= 0 || x_rows <= 0 || groups <= 0 || ksplit < 1 || ksplit > KB || (src == nullptr && x_rows < M)) return -1;
-  if (ldq % 16 || ldq < 128L * KB || lds < 4L * KB || ((uintptr_t)xq | (uintptr_t)qw) % 16 || (uintptr_t)ws % 4) return -1;
+  if (ldq % 128 || ldq < 128L * KB || lds < 4L * KB || ((uintptr_t)xq | (uintptr_t)qw) % 16 || (uintptr_t)ws % 4) return -1;
   if (epi == MX_GLU && (N % 256 || ksplit != 1 || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
   if (epi == MX_OUT && (ldo % 4 || ldo < N || (uintptr_t)out % 8 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;

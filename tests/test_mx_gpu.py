@@ -275,7 +275,7 @@ def gated_slack(xv, wv, bias, limit, alpha=1.702):
     return v, 1.1 * dg * (up + du) + f * du + 2.0 ** -20 * v.abs() + 1e-30
 
 
-@pytest.mark.parametrize("m", [1, 16, 19, 64, 100, 300])
+@pytest.mark.parametrize("m", [1, 16, 19, 64, 100, 300, 777])
 @pytest.mark.parametrize("inter,k,limit,bias", [(128, 128, 0.0, False), (256, 288, 7.0, True), (640, 1120, 0.0, True), (128, 4096, 7.0, False)])
 def test_gate_up(m, inter, k, limit, bias):
     from vllm_distributed_amd import ops

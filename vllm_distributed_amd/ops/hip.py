@@ -2519,8 +2519,19 @@ def _mx_check(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor
     return groups, nt, kb
 
 
-def mx_plan(m: int, n: int, kb: int) -> Tuple[int, int]:
-    """(16-row tiles a workgroup takes, K split)."""
+MX_BIG = 16                        # row_tiles of the kernel of 256-row tiles
+
+
+def mx_big_ok(rows: quant.MxRows, w: quant.MxWeight) -> bool:
+    """Whether the kernel of 256-row tiles takes these operands: both within 32-bit byte offsets."""
+    lim = (1 << 32) - 64
+    return rows.payload.numel() < lim and w.qw.shape[-4] * w.qw.shape[-3] * 1024 < lim
+
+
+def mx_plan(m: int, n: int, kb: int, big: bool = False) -> Tuple[int, int]:
+    """(16-row tiles a workgroup takes, K split); ``big``: the kernel of 256-row tiles may be chosen."""
+    if big and m > 512:
+        return MX_BIG, 1
     mt = 1 if m <= 16 else 2 if m <= 32 else 4
     wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
     return mt, max(1, min((512 + wgs - 1) // wgs, kb // 8))
@@ -2543,7 +2554,7 @@ def mx_linear(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor
     m = rows.shape[0]
     out = torch.empty((m, w.rows), dtype=rows.dtype, device=rows.device)
     if m:
-        mt, ksplit = mx_plan(m, w.rows, kb)
+        mt, ksplit = mx_plan(m, w.rows, kb, mx_big_ok(rows, w))
         partial = torch.empty((ksplit, m, w.rows), dtype=torch.float32, device=rows.device) if ksplit > 1 else None
         _mx_gemm(0, rows, w, bias, out, None, partial, ksplit, mt)
     return out
@@ -2571,7 +2582,7 @@ def mx_gate_up(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tenso
     r = _mx_gated_out(rows, w, m)
     _mx_check(rows, w, bias, False)
     if m:
-        _mx_gemm(2, rows, w, bias, r.payload, r.scales, None, 1, mx_plan(m, w.rows, 1)[0], limit, alpha)
+        _mx_gemm(2, rows, w, bias, r.payload, r.scales, None, 1, mx_plan(m, w.rows, 1, mx_big_ok(rows, w))[0], limit, alpha)
     return r
 
 
