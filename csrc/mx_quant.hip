@@ -6,16 +6,17 @@
 
 namespace {
 
-// rows of x [M][K] -> q [M][width of BITS], s [M][.]; columns K .. Kp are zeros
+// rows of x [M][K] (src: x[src[row]]) -> q [M][width of BITS], s [M][.]; columns K .. Kp are zeros
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s, long lds,
-                                                          const T* __restrict__ x, long ldx, long groups, int per_row, int K) {
+                                                          const T* __restrict__ x, long ldx, long groups, int per_row, int K,
+                                                          const int* __restrict__ src, int x_rows) {
   for (long i = blockIdx.x * 256L + threadIdx.x; i < groups; i += gridDim.x * 256L) {
     const long row = i / per_row;
     const int c = (int)(i - row * per_row);
     float v[8];
     if (8 * c < K) {                              // (whole blocks: a quad agrees)
-      mx_load8(x + row * ldx + 8 * c, v);
+      mx_load8(x + (src != nullptr ? (long)min(max(src[row], 0), x_rows - 1) : row) * ldx + 8 * c, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.f;
@@ -147,15 +148,17 @@ inline unsigned mx_blocks(long groups) {
 
 // x [M][K] (row stride ldx, a multiple of 8 elements, 16-byte aligned) -> q, s.  K % 32 == 0; q rows hold Kp >= K columns (a multiple
 // of 32; 1 byte each with 8 bits, half with 4), columns from K on zeros; s rows Kp / 32 bytes.
+// src [M] or null: row i is that of x [x_rows] that src names.
 VDAMD_API int vdamd_mx_quantize(void* q, long ldq, void* s, long lds, const void* x, long ldx, long M, int K, int Kp, int bits,
-                                int dtype, void* stream) {
+                                const int* src, int x_rows, int dtype, void* stream) {
   if (M <= 0) return 0;
+  if (src != nullptr && x_rows <= 0) return -1;
   if (K <= 0 || K % 32 || Kp < K || Kp % 32 || ldx % 8 || ldx < K || (uintptr_t)x % 16 || (uintptr_t)q % 16 || lds < Kp / 32) return -1;
   if ((bits != 8 && bits != 4) || ldq % 16 || ldq < (bits == 8 ? Kp : Kp / 2)) return -1;
   const int per_row = Kp / 8;
   const long groups = M * per_row;
   hipStream_t st = (hipStream_t)stream;
-#define GO(T, B) mx_quantize_kernel<T, B><<<mx_blocks(groups), 256, 0, st>>>((uint8_t*)q, ldq, (uint8_t*)s, lds, (const T*)x, ldx, groups, per_row, K)
+#define GO(T, B) mx_quantize_kernel<T, B><<<mx_blocks(groups), 256, 0, st>>>((uint8_t*)q, ldq, (uint8_t*)s, lds, (const T*)x, ldx, groups, per_row, K, src, x_rows)
   if (dtype == DT_BF16) { if (bits == 8) GO(bf16_t, 8); else GO(bf16_t, 4); }
   else if (dtype == DT_F16) { if (bits == 8) GO(f16_t, 8); else GO(f16_t, 4); }
   else if (dtype == DT_F32) { if (bits == 8) GO(float, 8); else GO(float, 4); }

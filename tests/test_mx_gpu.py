@@ -312,7 +312,7 @@ def make_experts(e, n, k, halves=1):
 
 
 @pytest.mark.parametrize("t,e,k,h,inter,limit", [(1, 8, 2, 128, 128, 0.0), (16, 128, 4, 288, 160, 7.0), (9, 4, 4, 160, 128, 7.0),
-                                                 (70, 8, 2, 256, 384, 0.0), (300, 5, 3, 96, 96, 7.0), (1200, 4, 2, 256, 128, 0.0)])
+                                                 (70, 8, 2, 256, 384, 0.0), (300, 5, 3, 96, 96, 7.0), (1200, 4, 2, 256, 128, 0.0), (513, 3, 2, 160, 416, 7.0)])
 def test_experts(t, e, k, h, inter, limit):
     from vllm_distributed_amd import ops
     from vllm_distributed_amd.ops import quant
@@ -346,16 +346,18 @@ def test_experts(t, e, k, h, inter, limit):
     assert off.norm() <= 2.0 ** -6 * want.norm()
 
 
-def test_experts_of_two_ranks_add_up():
+@pytest.mark.parametrize("t", [5, 33, 700])
+def test_experts_of_two_ranks_add_up(t):
     """Expert parallel: each rank adds its experts' part; in one row's 32-bit sum the parts are those of the whole block."""
     from vllm_distributed_amd import ops
-    t, e, k, h, inter = 33, 6, 3, 128, 128
+    e, k, h, inter = 6, 3, 128, 128
     x = rows(t, h, spread=0.3).cuda()
     w13, _ = make_experts(e, 2 * inter, h, halves=2)
     w2, _ = make_experts(e, h, inter)
     topi = torch.stack([torch.randperm(e)[:k] for _ in range(t)]).int().cuda()
     topw = torch.rand(t, k).cuda()
     whole = ops.mx_experts(x, topw, topi, w13, w2)
+    assert torch.equal(ops.mx_experts(ops.mx_quantize(x), topw, topi, w13, w2), whole)      # (rows that are 8-bit already)
     parts = []
     for lo in (0, 3):
         sl = lambda w: ops.MxWeight(w.qw[lo:lo + 3].contiguous(), w.ws[lo:lo + 3].contiguous(), w.rows)  # noqa: E731

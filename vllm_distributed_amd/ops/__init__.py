@@ -592,21 +592,27 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
     matrices are those of experts ``expert_start ..``, other slots add nothing; ``num_experts``: the router's outputs then."""
     e_local = weight13.qw.shape[0]
     total = num_experts or (e_local if local_experts < 0 else expert_start + local_experts)
-    rows = _mx_operand(x, weight13)
     t, k = topi.shape
-    if rows.shape[0] != t or topw.shape != topi.shape:
-        raise ValueError(f"{rows.shape[0]} rows, choices {tuple(topi.shape)}, weights {tuple(topw.shape)}")
+    if len(x.shape) != 2 or x.shape[0] != t or topw.shape != topi.shape:
+        raise ValueError(f"rows {tuple(x.shape)}, choices {tuple(topi.shape)}, weights {tuple(topw.shape)}")
+    dtype = x.dtype
     if local_experts >= 0 and not num_experts:
         raise ValueError("the number of the router's outputs is wanted beside local_experts")
     if local_experts >= 0 and local_experts != e_local or weight2.qw.shape[0] != e_local:
         raise ValueError(f"{e_local} and {weight2.qw.shape[0]} expert matrices, {local_experts} local experts")
-    if _mx_hip(rows.payload, rows.dtype) and t:
+    if _mx_hip(x.payload if isinstance(x, MxRows) else x, dtype) and t:
         tile_rows = _hip.mx_tile_rows(t * k, total)
+        if tile_rows == 256 and not (_hip.mx_sorted_ok(t * k, weight13) and _hip.mx_sorted_ok(t * k, weight2)):
+            tile_rows = 64
         src_row, inv, tiles = moe_align_fused(topi, total, tile_rows, expert_start, local_experts)
-        a = _hip.mx_grouped_gate_up(rows, weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
+        if tile_rows == 256:          # (large tiles read their rows in order: quantised, or gathered, into it)
+            rows, src_row = _hip.mx_sorted_rows(x, src_row), None
+        else:
+            rows = x if isinstance(x, MxRows) else _hip.mx_quantize(x, 8)
+        a = _hip.mx_grouped_gate_up(_mx_operand(rows, weight13), weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
         y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2)
         return moe_combine(y, topw, topi, inv, expert_start, local_experts)
-    return torch_ref.mx_experts(rows, topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)
+    return torch_ref.mx_experts(_mx_operand(x, weight13), topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)
 
 
 def moe_align(topi, num_experts: int, tile_rows: int, expert_start: int = 0, local_experts: int = -1):

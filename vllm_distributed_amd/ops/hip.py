@@ -96,7 +96,7 @@ def load() -> ctypes.CDLL:
         "vdamd_delta_rule_rows": [P, P, L, P, L, P, L] + [P] * 6 + [I] * 6 + [F, I, P],
         "vdamd_gated_delta_rule": [P, P, L, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
         "vdamd_embed_scaled": [P, P, P, F, I, I, I, I, P],
-        "vdamd_mx_quantize": [P, L, P, L, P, L, L, I, I, I, I, P],
+        "vdamd_mx_quantize": [P, L, P, L, P, L, L, I, I, I, P, I, I, P],
         "vdamd_mx_dequantize": [P, P, L, P, L, L, I, I, I, P],
         "vdamd_mx_rms_norm": [P, L, P, L, P, P, L, P, I, P, P, F, I, I, I, I, P],
         "vdamd_mx_gemm": [P, L, P, L, P, P, L, P, L, I, P, P, P, I, I, I, I, I, F, F, P, I, I, P, I, I, P],
@@ -2456,13 +2456,19 @@ def _mx_rows(x: torch.Tensor) -> torch.Tensor:
     return x2
 
 
-def mx_quantize(x: torch.Tensor, bits: int, dtype: Optional[torch.dtype] = None) -> quant.MxRows:
+def mx_quantize(x: torch.Tensor, bits: int, dtype: Optional[torch.dtype] = None, src_row: Optional[torch.Tensor] = None) -> quant.MxRows:
+    """``src_row``: of the rows ``x[src_row]``."""
     x2 = _mx_rows(x)
-    _mx_device(x.device, x2)
+    _mx_device(x.device, x2, src_row)
     m, k = x2.shape
+    rows = m
+    if src_row is not None:
+        assert src_row.dtype == torch.int32 and src_row.dim() == 1 and src_row.is_contiguous() and (m or not src_row.numel())
+        m = src_row.numel()
     r = quant.MxRows.empty(m, k, bits, dtype or x.dtype, x.device)
     _check(_LIB.vdamd_mx_quantize(r.payload.data_ptr(), r.payload.stride(0), r.scales.data_ptr(), r.scales.stride(0), x2.data_ptr(),
-                                  x2.stride(0), m, k, r.payload.shape[1] * 8 // bits, bits, _dt(x2), _stream()), "mx_quantize")
+                                  x2.stride(0), m, k, r.payload.shape[1] * 8 // bits, bits, _ptr(src_row), rows, _dt(x2), _stream()),
+           "mx_quantize")
     return r
 
 
@@ -2589,13 +2595,27 @@ def mx_gate_up(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tenso
 def mx_tile_rows(slots: int, experts: int) -> int:
     """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices."""
     avg = slots / max(1, experts)
-    return 16 if avg <= 16 else 32 if avg <= 32 else 64
+    return 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 96 else 256
+
+
+def mx_sorted_ok(slots: int, w: quant.MxWeight) -> bool:
+    """Whether ``slots`` rows of ``w``'s reduction, one after the other, and one of its matrices are within 32-bit byte offsets."""
+    lim = (1 << 32) - 64
+    return slots * w.qw.shape[-3] * 128 < lim and w.qw.shape[-4] * w.qw.shape[-3] * 1024 < lim
+
+
+def mx_sorted_rows(x, src_row: torch.Tensor) -> quant.MxRows:
+    """``x[src_row]`` in 8 bits, ``x`` 16-bit rows or ``MxRows``."""
+    if not isinstance(x, quant.MxRows):
+        return mx_quantize(x, 8, src_row=src_row)
+    return quant.MxRows(x.payload.index_select(0, src_row), x.scales.index_select(0, src_row), x.width, x.bits, x.dtype)
 
 
 def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], device: torch.device) -> int:
     assert tiles.dtype == torch.int32 and tiles.dim() == 2 and tiles.shape[1] == 3 and tiles.is_contiguous()
     assert src is None or (src.dtype == torch.int32 and src.dim() == 1 and src.is_contiguous())
-    assert tile_rows in (16, 32, 64), tile_rows
+    assert tile_rows in (16, 32, 64, 256), tile_rows
+    assert tile_rows < 256 or src is None, "tiles of 256 rows: the rows themselves, in order"
     _mx_device(device, tiles, src)
     return tile_rows // 16
 
