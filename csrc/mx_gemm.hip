@@ -206,12 +206,14 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
 //    x; the 16-byte slots of a row XOR-ed with (row >> 1) & 7 at the source, so that the lanes of a fragment read meet no bank twice)
 //    and B0, B1 (eight weight tiles of 1 KiB, in the order in which lanes read them).  Two sets of images.
 //  * A wave has 128 x 64 outputs as four quadrants of 64 x 32, quadrant (mq, nq) from images A<mq> and B<nq>; a step is four phases of
-//    eight matrix instructions, one quadrant each, every fragment read once: A0 in phase 0, A1 in 1, B1 in 2, the next step's B0 in 3.
-//  * The loads are one stream that never drains: image h = 4 t + (A0, B0, A1, B1) is issued in phase h - 6, and a phase waits until all
-//    but the newest four images (three in phase 2, ahead of the early read) are there: 6 and 5 loads, an A image being two loads of a
-//    wave and a B image one.  It runs on through the output tiles.
-//  * Scales come 16 bytes a row (four steps) at a time into two further sets, one load of each wave in every other step, at its third
-//    phase: one more in the counts from there to its sixth.  Lanes read their byte from LDS.
+//    eight matrix instructions, one quadrant each, every fragment read once.  Even steps go A0 B0, A1 B0, A1 B1, A0 B1, odd ones begin
+//    with A1: registers of the half that a step begins with are free a phase before it, so the 20 fragment reads of a step spread as
+//    6, 6, 4, 4 over its phases and stay below the matrix instructions' time in each (as 8, 8, 2, 2: 2780 TFLOP/s instead of ____).
+//  * The loads are one stream that never drains.  Of step t are issued: B0 in phase 1 of step t - 2, the first A half in 2, the second in
+//    3, B1 in phase 0 of step t - 1; each at least two phases after the image before it was read.  A phase waits for what the next one
+//    reads, all but the newest six loads of a wave (an A image is two, a B image one).  It runs on through the output tiles.
+//  * Scales come 16 bytes a row (four steps) at a time into two further sets, one load of each wave in every other step, at its phase 1:
+//    one more in the counts until they are older.  Lanes read their byte from LDS.
 //  * Waves 4-7 run one barrier behind waves 0-3: on each SIMD one wave multiplies while the other reads.
 //  * An odd number of steps gets one more, whose weights are zeros: loads out of the descriptor's range.
 constexpr int MXB_A = 128 * 128, MXB_B = 8 * 1024, MXB_SET = 2 * MXB_A + 2 * MXB_B, MXB_SC = 2 * 4096;
@@ -316,12 +318,12 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
   const int swz = (r16 >> 1) & 7, so0 = (q ^ swz) << 4, so1 = ((4 + q) ^ swz) << 4;
   const int xro = (wr * 64 + r16) * 128, wro = 2 * MXB_A + wc * 2048 + lane * 16;
   const int xso = 2 * MXB_SET + (wr * 64 + r16) * 16 + q, wso = 2 * MXB_SET + 4096 + wc * 512 + lane * 4;
-  auto read_x = [&](mx_i32x8 (&f)[4], uint32_t (&s)[4], int set, int half, int sbyte) {
+  auto read_x = [&](mx_i32x8 (&f)[4], uint32_t (&s)[4], int from, int to, int set, int half, int sbyte) {
     const unsigned char* b = smem + set * MXB_SET + half * MXB_A + xro;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = mx_fragment(b + i * 2048 + so0, b + i * 2048 + so1);
+    for (int i = from; i < to; ++i) f[i] = mx_fragment(b + i * 2048 + so0, b + i * 2048 + so1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = smem[xso + sbyte + half * 2048 + i * 256];
+    for (int i = from; i < to; ++i) s[i] = smem[xso + sbyte + half * 2048 + i * 256];
   };
   auto read_w = [&](mx_u32x4 (&f)[2], uint32_t (&s)[2], int set, int half, int sbyte, int step) {
     const unsigned char* b = smem + set * MXB_SET + half * MXB_B + wro;
@@ -362,8 +364,8 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
   srs = scales(cur.g);
   int par = 0;                               // which set holds the scales of the current four steps
   stage_s(0, 0);
-  stage_a(0, 0, 0); stage_b(0, 0, 0); stage_a(1, 0, 0); stage_b(1, 0, 0);
-  stage_a(0, 1, 1); stage_b(0, 1, 1);
+  stage_b(0, 0, 0); stage_a(0, 0, 0); stage_a(1, 0, 0); stage_b(1, 0, 0);
+  stage_b(0, 1, 1); stage_a(1, 1, 1); stage_a(0, 1, 1);
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -371,6 +373,7 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
   if (wr == 1) __builtin_amdgcn_s_barrier();          // waves 4-7 run one barrier behind
   __builtin_amdgcn_sched_barrier(0);
   read_w(wf0, sw0, 0, 0, 0, 0);
+  read_x(xf0, sx0, 0, 2, 0, 0, 0);
 
   for (;;) {
     const int next = used(tile + stride);
@@ -392,8 +395,8 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
       const int s0 = min(t, KB - 1) & 3, s1 = min(t + 1, KB - 1) & 3;      // (the step of zeros takes its neighbour's scales)
       const bool last = t == KT - 2;
       const int now = par * MXB_SC;
-      MXB_PHASE(read_x(xf0, sx0, 0, 0, now + 4 * s0), stage_a(1, 1, t + 1), 6, acc00, xf0, sx0, wf0, sw0)
-      MXB_PHASE(read_x(xf1, sx1, 0, 1, now + 4 * s0), stage_b(1, 1, t + 1), 6, acc10, xf1, sx1, wf0, sw0)
+      // the even step: A0 B0, A1 B0, A1 B1, A0 B1
+      MXB_PHASE(read_x(xf0, sx0, 2, 4, 0, 0, now + 4 * s0); read_x(xf1, sx1, 0, 1, 0, 1, now + 4 * s0), stage_b(1, 1, t + 1), 7, acc00, xf0, sx0, wf0, sw0)
       cur.rows = last ? nxt.rows : cur.rows;
       cur.b0 = last ? nxt.b0 : cur.b0;
       cur.b1 = last ? nxt.b1 : cur.b1;
@@ -403,13 +406,16 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
         wrs = weights(cur.g);
         srs = scales(cur.g);
       }
-      MXB_PHASE(read_w(wf1, sw1, 0, 1, now, s0), stage_s(par ^ 1, last ? 0 : (t >> 2) + 1); stage_a(0, 0, t + 2), 6, acc11, xf1, sx1, wf1, sw1)
-      MXB_PHASE(read_w(wf0, sw0, 1, 0, now, s1), stage_b(0, 0, t + 2), 7, acc01, xf0, sx0, wf1, sw1)
-      MXB_PHASE(read_x(xf0, sx0, 1, 0, now + 4 * s1), stage_a(1, 0, t + 2), 7, acc00, xf0, sx0, wf0, sw0)
-      MXB_PHASE(read_x(xf1, sx1, 1, 1, now + 4 * s1), stage_b(1, 0, t + 2), 7, acc10, xf1, sx1, wf0, sw0)
+      MXB_PHASE(read_x(xf1, sx1, 1, 4, 0, 1, now + 4 * s0), stage_s(par ^ 1, last ? 0 : (t >> 2) + 1); stage_b(0, 0, t + 2), 7, acc10, xf1, sx1, wf0, sw0)
+      MXB_PHASE(read_w(wf1, sw1, 0, 1, now, s0); read_w(wf0, sw0, 1, 0, now, s1), stage_a(0, 0, t + 2), 7, acc11, xf1, sx1, wf1, sw1)
+      MXB_PHASE(read_x(xf1, sx1, 0, 2, 1, 1, now + 4 * s1), stage_a(1, 0, t + 2), 7, acc01, xf0, sx0, wf1, sw1)
+      // the odd one: A1 B0, A0 B0, A0 B1, A1 B1
+      MXB_PHASE(read_x(xf1, sx1, 2, 4, 1, 1, now + 4 * s1); read_x(xf0, sx0, 0, 1, 1, 0, now + 4 * s1), stage_b(1, 0, t + 2), 7, acc10, xf1, sx1, wf0, sw0)
+      MXB_PHASE(read_x(xf0, sx0, 1, 4, 1, 0, now + 4 * s1), stage_b(0, 1, t + 3), 6, acc00, xf0, sx0, wf0, sw0)
       par ^= (int)(last || (t & 2));
-      MXB_PHASE(read_w(wf1, sw1, 1, 1, now, s1), stage_a(0, 1, t + 3), 5, acc11, xf1, sx1, wf1, sw1)
-      MXB_PHASE(read_w(wf0, sw0, 0, 0, par * MXB_SC, last ? 0 : (t + 2) & 3), stage_b(0, 1, t + 3), 6, acc01, xf0, sx0, wf1, sw1)
+      const int then = par * MXB_SC, s2 = last ? 0 : (t + 2) & 3;
+      MXB_PHASE(read_w(wf1, sw1, 1, 1, now, s1); read_w(wf0, sw0, 0, 0, then, s2), stage_a(1, 1, t + 3), 6, acc01, xf0, sx0, wf1, sw1)
+      MXB_PHASE(read_x(xf0, sx0, 0, 2, 0, 0, then + 4 * s2), stage_a(0, 1, t + 3), 6, acc11, xf1, sx1, wf1, sw1)
     }
     // nothing below may be computed before the K loop (it would be live across it)
     asm volatile("" : "+s"(cm0), "+s"(ctn), "+s"(cend), "+s"(cg));
@@ -437,18 +443,25 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
           mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n, a.os + (long)m * a.ldos + (n >> 5), v, eln, m < cend);
         } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            const int nb = 256 * ctn + 128 * h + 32 * wc;
+            mx_u32x2 pk[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const int n = 256 * ctn + 128 * h + 32 * wc + 16 * j + 4 * eq;
+              const int n = nb + 16 * j + 4 * eq;
               const f32x4 v = h ? a1[i][j] : a0[i][j];
-              if (m < cend && n < a.N) {
-                typename Vec4<T>::type o;
+              typename Vec4<T>::type o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (T)(v[e] + (bias ? (float)bias[n + e] : 0.f));
-                *reinterpret_cast<typename Vec4<T>::type*>((T*)a.out + (long)m * a.ldo + n) = o;
-              }
+              for (int e = 0; e < 4; ++e) o[e] = (T)(v[e] + (bias != nullptr && n < a.N ? (float)bias[n + e] : 0.f));
+              pk[j] = __builtin_bit_cast(mx_u32x2, o);
             }
+            // lanes of even q trade their second fragment's columns for the next lane's first: 16 bytes each, 64 neighbouring a row
+            const auto p0 = __builtin_amdgcn_permlane16_swap(pk[0][0], pk[1][0], false, false);
+            const auto p1 = __builtin_amdgcn_permlane16_swap(pk[0][1], pk[1][1], false, false);
+            const int n = nb + ((eq & 1) ? 16 + 4 * (eq - 1) : 4 * eq);
+            if (m < cend && n < a.N)
+              *reinterpret_cast<mx_u32x4*>((T*)a.out + (long)m * a.ldo + n) = mx_u32x4{(uint32_t)p0[0], (uint32_t)p1[0], (uint32_t)p0[1], (uint32_t)p1[1]};
+          }
         }
       }
     };
@@ -555,7 +568,7 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
   if (N <= 0 || N % 8 || KB <= 0 || x_rows <= 0 || groups <= 0 || ksplit < 1 || ksplit > KB || (src == nullptr && x_rows < M)) return -1;
   if (ldq % 128 || ldq < 128L * KB || lds < 4L * KB || ((uintptr_t)xq | (uintptr_t)qw) % 16 || (uintptr_t)ws % 4) return -1;
   if (epi == MX_GLU && (N % 256 || ksplit != 1 || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
-  if (epi == MX_OUT && (ldo % 4 || ldo < N || (uintptr_t)out % 8 || (ksplit > 1 && partial == nullptr))) return -1;
+  if (epi == MX_OUT && (ldo % 8 || ldo < N || (uintptr_t)out % 16 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;
   if ((ksplit > 1 || epi == MX_SLAB) && tiles != nullptr) return -1;
   if (epi < 0 || epi > 2) return -1;
