@@ -200,6 +200,42 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
   }
 }
 
+// The bias of 32 columns from n0 (the same for the wave) for a lane with columns 16 j + 4 q .. + 3 of them: by scalar loads, since a vector
+// load could only be waited for together with everything in flight.  Columns from N on: zeros
+template <typename T>
+__device__ __forceinline__ void mx_bias(float (&b)[2][4], const void* bias, long group, int n0, int N, int q) {
+  typedef const __attribute__((address_space(4))) uint32_t* words;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[j][e] = 0.f;
+  if (bias == nullptr) return;
+  const T* p = (const T*)bias + group;
+  if (n0 + 32 <= N) {
+    words w = (words)(uintptr_t)(p + n0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v = w[8 * j + h];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) v = q == i ? w[8 * j + 2 * i + h] : v;
+        typedef T pair __attribute__((ext_vector_type(2)));
+        const pair t = __builtin_bit_cast(pair, v);
+        b[j][2 * h] = (float)t[0];
+        b[j][2 * h + 1] = (float)t[1];
+      }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + 16 * j + 4 * q + e;
+        if (n < N) b[j][e] = (float)p[n];
+      }
+  }
+}
+
 // Many rows: the matrix cores are the time.  256 x 256 outputs a tile (MX_GLU: 128 columns of the gate and the same of the up half), one
 // persistent workgroup of eight waves a compute unit, K in steps of 128.
 //  * Both operands go from memory to LDS without passing through registers.  A step is four images: A0, A1 (128 rows x 128 bytes of
@@ -424,41 +460,38 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
     int eln = lane;
     asm volatile("" : "+v"(eln));
     const int er = eln & 15, eq = eln >> 4;
+    // (MX_OUT: the second group of 32 columns is 128 on, MX_GLU: in the up half)
+    const int n0 = EPI == MX_GLU ? 128 * ctn + 32 * wc : 256 * ctn + 32 * wc, n1 = n0 + (EPI == MX_GLU ? a.N >> 1 : 128);
+    float b0[2][4], b1[2][4];
+    mx_bias<T>(b0, a.bias, (long)cg * a.N, n0, a.N, eq);
+    mx_bias<T>(b1, a.bias, (long)cg * a.N, n1, a.N, eq);
     auto put = [&](const f32x4 (&a0)[4][2], const f32x4 (&a1)[4][2], int mq) {
-      const T* bias = a.bias == nullptr ? nullptr : (const T*)a.bias + (long)cg * a.N;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int m = cm0 + 128 * mq + 64 * wr + 16 * i + er;
         if constexpr (EPI == MX_GLU) {
-          const int half = a.N >> 1, n = 128 * ctn + 32 * wc;
           float v[2][4];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int c = n + 16 * j + 4 * eq + e;
-              v[j][e] = mx_glu(a0[i][j][e] + (bias ? (float)bias[c] : 0.f), a1[i][j][e] + (bias ? (float)bias[half + c] : 0.f),
-                               a.limit, a.alpha);
-            }
-          mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n, a.os + (long)m * a.ldos + (n >> 5), v, eln, m < cend);
+            for (int e = 0; e < 4; ++e) v[j][e] = mx_glu(a0[i][j][e] + b0[j][e], a1[i][j][e] + b1[j][e], a.limit, a.alpha);
+          mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n0, a.os + (long)m * a.ldos + (n0 >> 5), v, eln, m < cend);
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int nb = 256 * ctn + 128 * h + 32 * wc;
             mx_u32x2 pk[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const int n = nb + 16 * j + 4 * eq;
               const f32x4 v = h ? a1[i][j] : a0[i][j];
               typename Vec4<T>::type o;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[e] = (T)(v[e] + (bias != nullptr && n < a.N ? (float)bias[n + e] : 0.f));
+              for (int e = 0; e < 4; ++e) o[e] = (T)(v[e] + (h ? b1[j][e] : b0[j][e]));
               pk[j] = __builtin_bit_cast(mx_u32x2, o);
             }
             // lanes of even q trade their second fragment's columns for the next lane's first: 16 bytes each, 64 neighbouring a row
             const auto p0 = __builtin_amdgcn_permlane16_swap(pk[0][0], pk[1][0], false, false);
             const auto p1 = __builtin_amdgcn_permlane16_swap(pk[0][1], pk[1][1], false, false);
-            const int n = nb + ((eq & 1) ? 16 + 4 * (eq - 1) : 4 * eq);
+            const int n = (h ? n1 : n0) + ((eq & 1) ? 16 + 4 * (eq - 1) : 4 * eq);
             if (m < cend && n < a.N)
               *reinterpret_cast<mx_u32x4*>((T*)a.out + (long)m * a.ldo + n) = mx_u32x4{(uint32_t)p0[0], (uint32_t)p1[0], (uint32_t)p0[1], (uint32_t)p1[1]};
           }
@@ -566,7 +599,7 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
                             int dtype, void* stream) {
   if (M <= 0 || (tiles != nullptr && num_tiles <= 0)) return 0;
   if (N <= 0 || N % 8 || KB <= 0 || x_rows <= 0 || groups <= 0 || ksplit < 1 || ksplit > KB || (src == nullptr && x_rows < M)) return -1;
-  if (ldq % 128 || ldq < 128L * KB || lds < 4L * KB || ((uintptr_t)xq | (uintptr_t)qw) % 16 || (uintptr_t)ws % 4) return -1;
+  if (ldq % 128 || ldq < 128L * KB || lds < 4L * KB || ((uintptr_t)xq | (uintptr_t)qw) % 16 || ((uintptr_t)ws | (uintptr_t)bias) % 4) return -1;
   if (epi == MX_GLU && (N % 256 || ksplit != 1 || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
   if (epi == MX_OUT && (ldo % 8 || ldo < N || (uintptr_t)out % 16 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;

@@ -74,7 +74,7 @@ def test_quantize(bits, dtype, m, k):
     assert torch.equal(r.s.view(torch.uint8).cpu().long(), byte)
     got = r.q.view(torch.uint8).cpu()
     assert torch.equal(got.long(), code) if bits == 8 else torch.equal(got, oracle.pack4(code))
-    assert not r.payload[:, k * bits // 8:].any()                      # the padding is zeros
+    assert not r.payload.view(torch.uint8)[:, k * bits // 8:].any()                      # the padding is zeros
     assert torch.equal(ops.mx_dequantize(r, torch.float32).cpu().double(), value.float().double())
 
 
@@ -163,7 +163,7 @@ def test_norm(dtype, m, h, form):
     # 32-bit arithmetic: a sum of h squares in at most 10 + log2(1024) dependent additions, root, division, two products, each 2^-24
     size = (slabs.double().abs().sum(0) + residual.double().abs()) / total.abs().clamp_min(1e-30) if form == "slabs" else torch.ones_like(v)
     check_rows(r, v, (40 + 4 * size) * 2.0 ** -24 * v.abs())
-    assert not r.payload[:, h:].any()
+    assert not r.payload.view(torch.uint8)[:, h:].any()
 
 
 def test_norm_keeps_its_inputs_and_takes_strides():
@@ -174,7 +174,7 @@ def test_norm_keeps_its_inputs_and_takes_strides():
     r, out = ops.fused_add_rms_norm_mx(x, residual, gain, 1e-6)
     assert torch.equal(wide, before[0]) and torch.equal(residual, before[1])
     again, out2 = ops.fused_add_rms_norm_mx(x.contiguous(), residual, gain, 1e-6)
-    assert torch.equal(r.payload, again.payload) and torch.equal(r.s.view(torch.uint8), again.s.view(torch.uint8)) and torch.equal(out, out2)
+    assert torch.equal(r.payload.view(torch.uint8), again.payload.view(torch.uint8)) and torch.equal(r.s.view(torch.uint8), again.s.view(torch.uint8)) and torch.equal(out, out2)
 
 
 # ------------------------------------------------------------------ products

@@ -500,13 +500,14 @@ def mx_quantize(x, bits: int = 8) -> MxRows:
     """Rows ``x [.., K]`` (16- or 32-bit floats, ``K % 32 == 0``) in microscaled floating point: elements of 8 (e4m3) or 4 (e2m1) bits,
     a power of two for each 32 neighbours - the smallest that keeps every element within the format, so none saturates; elements
     to nearest, ties to even.  A block with a NaN or an infinity becomes NaN as a whole."""
-    if bits not in (4, 8):
-        raise ValueError(f"microscaled rows hold 8 or 4 bits a value, not {bits}")
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"mx_quantize of {x.dtype}")
+    if _use_hip(x):
+        return _hip.mx_quantize(x, bits)
+    if bits not in (4, 8):
+        raise ValueError(f"microscaled rows hold 8 or 4 bits a value, not {bits}")
     _mx_width(x.shape[-1])
-    x2 = x.reshape(-1, x.shape[-1])
-    return _hip.mx_quantize(x2, bits) if _use_hip(x2) else quant.mx_quantize(x2, bits)
+    return quant.mx_quantize(x.reshape(-1, x.shape[-1]), bits)
 
 
 def mx_dequantize(rows: MxRows, dtype: Optional[torch.dtype] = None):

@@ -2437,19 +2437,20 @@ def gated_unit_step(u, ra, ra_bias, ri, ri_bias, rate, gate, gate_bias, state, s
 MX_NORM_MAX = 32768
 
 
-def _mx_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    """The kernels are launched on the current device's current stream: every operand has to be there."""
+def _mx_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels are launched on the current device's current stream: every operand has to be there (``dev``: the first one's)."""
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"operands on {device} and on {t.device}")
-    if device.index is not None and device.index != torch.cuda.current_device():
-        raise ValueError(f"operands on {device}, current device cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"operands on device {dev} and on {t.device}")
+    if dev != (torch.cuda.current_device() if _current_device is None else _current_device()):
+        raise ValueError(f"operands on cuda:{dev}, current device cuda:{torch.cuda.current_device()}")
 
 
 def _mx_rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` as rows that the kernels can read: unit stride, 16-byte borders."""
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    s0, s1 = x2.stride()
+    if s1 != 1 or s0 % 8 or s0 < x2.shape[1] or x2.data_ptr() % 16:
         x2 = x2.contiguous()
         if x2.data_ptr() % 16:
             x2 = x2.clone()
@@ -2459,79 +2460,87 @@ def _mx_rows(x: torch.Tensor) -> torch.Tensor:
 def mx_quantize(x: torch.Tensor, bits: int, dtype: Optional[torch.dtype] = None, src_row: Optional[torch.Tensor] = None) -> quant.MxRows:
     """``src_row``: of the rows ``x[src_row]``."""
     x2 = _mx_rows(x)
-    _mx_device(x.device, x2, src_row)
     m, k = x2.shape
     rows = m
     if src_row is not None:
         assert src_row.dtype == torch.int32 and src_row.dim() == 1 and src_row.is_contiguous() and (m or not src_row.numel())
         m = src_row.numel()
-    r = quant.MxRows.empty(m, k, bits, dtype or x.dtype, x.device)
-    _check(_LIB.vdamd_mx_quantize(r.payload.data_ptr(), r.payload.stride(0), r.scales.data_ptr(), r.scales.stride(0), x2.data_ptr(),
-                                  x2.stride(0), m, k, r.payload.shape[1] * 8 // bits, bits, _ptr(src_row), rows, _dt(x2), _stream()),
-           "mx_quantize")
+    _mx_device(x2.get_device(), src_row)
+    r = quant.MxRows.empty(m, k, bits, dtype or x.dtype, x2.device)
+    q, s = r.payload, r.scales
+    ldq = q.shape[1]
+    _check(_LIB.vdamd_mx_quantize(q.data_ptr(), ldq, s.data_ptr(), s.shape[1], x2.data_ptr(), x2.stride(0), m, k, ldq * 8 // bits, bits,
+                                  None if src_row is None else src_row.data_ptr(), rows, _dt(x2), _stream()), "mx_quantize")
     return r
 
 
 def mx_dequantize(rows: quant.MxRows, dtype: torch.dtype) -> torch.Tensor:
-    _mx_device(rows.device, rows.payload, rows.scales)
+    q, s = rows.payload, rows.scales
+    _mx_device(q.get_device(), s)
     m, k = rows.shape
-    out = torch.empty((m, k), dtype=dtype, device=rows.device)
-    _check(_LIB.vdamd_mx_dequantize(out.data_ptr(), rows.payload.data_ptr(), rows.payload.stride(0), rows.scales.data_ptr(),
-                                    rows.scales.stride(0), m, k, rows.bits, _dt(out), _stream()), "mx_dequantize")
+    out = torch.empty((m, k), dtype=dtype, device=q.device)
+    _check(_LIB.vdamd_mx_dequantize(out.data_ptr(), q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1], m, k, rows.bits, _dt(out),
+                                    _stream()), "mx_dequantize")
     return out
 
 
 def mx_rms_norm(x: Optional[torch.Tensor], slabs: Optional[torch.Tensor], residual: Optional[torch.Tensor], weight: torch.Tensor,
                 eps: float) -> Tuple[quant.MxRows, Optional[torch.Tensor]]:
     """``x [M, H]`` or fp32 slabs ``[ks, M, H]`` of it; returns the normed rows and the new residual (None without one)."""
-    h = weight.numel()
+    h, dtype, dev = weight.numel(), weight.dtype, weight.get_device()
+    ldx = ks = 0
+    x2 = None
     if slabs is not None:
         assert slabs.dtype == torch.float32 and slabs.dim() == 3 and slabs.is_contiguous() and slabs.shape[2] == h
-        m, x2 = slabs.shape[1], None
+        ks, m, _ = slabs.shape
     else:
         x2 = _mx_rows(x)
-        m = x2.shape[0]
-        assert x2.shape[1] == h and x2.dtype == weight.dtype, (x.shape, x.dtype, weight.shape, weight.dtype)
+        m, ldx = x2.shape[0], x2.stride(0)
+        assert x2.shape[1] == h and x2.dtype == dtype, (x.shape, x.dtype, weight.shape, dtype)
     assert _half(weight) and weight.is_contiguous() and weight.data_ptr() % 16 == 0
     assert h % 32 == 0 and h <= MX_NORM_MAX, f"rows of {h} values: multiples of 32 up to {MX_NORM_MAX} are normed into blocks"
     out = None
     if residual is not None:
-        assert residual.dtype == weight.dtype and residual.numel() == m * h and residual.shape[-1] == h
+        assert residual.dtype == dtype and residual.numel() == m * h and residual.shape[-1] == h
         residual = residual.contiguous()
         out = torch.empty_like(residual)
-    _mx_device(weight.device, x2, slabs, residual)
-    r = quant.MxRows.empty(m, h, 8, weight.dtype, weight.device)
-    _check(_LIB.vdamd_mx_rms_norm(r.payload.data_ptr(), r.payload.stride(0), r.scales.data_ptr(), r.scales.stride(0), _ptr(out),
-                                  _ptr(x2), 0 if x2 is None else x2.stride(0), _ptr(slabs), 0 if slabs is None else slabs.shape[0],
-                                  _ptr(residual), weight.data_ptr(), float(eps), m, h, r.payload.shape[1], _dt(weight), _stream()),
-           "mx_rms_norm")
+    _mx_device(dev, x2, slabs, residual)
+    r = quant.MxRows.empty(m, h, 8, dtype, weight.device)
+    q, s = r.payload, r.scales
+    ldq = q.shape[1]
+    _check(_LIB.vdamd_mx_rms_norm(q.data_ptr(), ldq, s.data_ptr(), s.shape[1], _ptr(out), _ptr(x2), ldx, _ptr(slabs), ks, _ptr(residual),
+                                  weight.data_ptr(), eps, m, h, ldq, _DT[dtype], _stream()), "mx_rms_norm")
     return r, out
 
 
 def _mx_check(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor], grouped: bool) -> Tuple[int, int, int]:
-    """(matrices, rows of each, 128-column steps) of a weight that ``rows`` can be multiplied with."""
-    d = 5 if grouped else 4
-    assert rows.bits == 8 and rows.dtype in (torch.bfloat16, torch.float16), (rows.bits, rows.dtype)
-    assert w.qw.dim() == d and w.qw.dtype == torch.int32 and w.qw.is_contiguous() and tuple(w.qw.shape[-2:]) == (64, 4)
-    nt, kb = w.qw.shape[-4:-2]
-    assert w.ws.dtype == torch.uint8 and w.ws.is_contiguous() and tuple(w.ws.shape) == (*w.qw.shape[:-4], nt, (kb + 3) // 4, 64, 4)
-    assert nt == (w.rows + 15) // 16 and w.rows % 8 == 0 and w.rows > 0
-    assert rows.payload.shape[1] == 128 * kb, f"rows of {rows.width} columns, a weight of {128 * kb} with padding"
-    assert rows.payload.is_contiguous() and rows.scales.is_contiguous() and rows.scales.shape[1] >= 4 * kb
-    groups = w.qw.shape[0] if grouped else 1
+    """(matrices, 16-row tiles of each, 128-column steps) of a weight that ``rows`` can be multiplied with."""
+    qw, ws, n = w
+    q, s, dtype = rows.payload, rows.scales, rows.dtype
+    assert rows.bits == 8 and (dtype == torch.bfloat16 or dtype == torch.float16), (rows.bits, dtype)
+    shape = qw.shape
+    assert len(shape) == (5 if grouped else 4) and shape[-1] == 4 and shape[-2] == 64 and qw.dtype == torch.int32 and qw.is_contiguous()
+    nt, kb = shape[-4], shape[-3]
+    assert ws.shape == (*shape[:-4], nt, (kb + 3) // 4, 64, 4) and ws.dtype == torch.uint8 and ws.is_contiguous(), (ws.shape, shape)
+    assert n > 0 and n % 8 == 0 and nt == (n + 15) // 16, (n, nt)
+    m = q.shape[0]
+    assert q.shape[1] == 128 * kb, f"rows of {rows.width} columns, a weight of {128 * kb} with padding"
+    assert q.is_contiguous() and s.is_contiguous() and s.shape == (m, (kb + 3) // 4 * 16), (q.shape, s.shape)
+    groups = shape[0] if grouped else 1
     if bias is not None:
-        assert bias.dtype == rows.dtype and bias.is_contiguous() and tuple(bias.shape) == ((groups, w.rows) if grouped else (w.rows,))
-    _mx_device(rows.device, rows.payload, rows.scales, w.qw, w.ws, bias)
+        assert bias.dtype == dtype and bias.is_contiguous() and bias.data_ptr() % 4 == 0, (bias.dtype, dtype)
+        assert bias.shape == ((groups, n) if grouped else (n,)), (bias.shape, groups, n)
+    _mx_device(q.get_device(), s, qw, ws, bias)
     return groups, nt, kb
 
 
 MX_BIG = 16                        # row_tiles of the kernel of 256-row tiles
 
 
-def mx_big_ok(rows: quant.MxRows, w: quant.MxWeight) -> bool:
-    """Whether the kernel of 256-row tiles takes these operands: both within 32-bit byte offsets."""
+def mx_big_ok(m: int, nt: int, kb: int) -> bool:
+    """Whether the kernel of 256-row tiles takes ``m`` rows and a matrix of ``nt`` tiles: both within 32-bit byte offsets."""
     lim = (1 << 32) - 64
-    return rows.payload.numel() < lim and w.qw.shape[-4] * w.qw.shape[-3] * 1024 < lim
+    return m * kb * 128 < lim and nt * kb * 1024 < lim
 
 
 def mx_plan(m: int, n: int, kb: int, big: bool = False) -> Tuple[int, int]:
@@ -2543,52 +2552,51 @@ def mx_plan(m: int, n: int, kb: int, big: bool = False) -> Tuple[int, int]:
     return mt, max(1, min((512 + wgs - 1) // wgs, kb // 8))
 
 
-def _mx_gemm(epi: int, rows: quant.MxRows, w: quant.MxWeight, bias, out, os, partial, ksplit: int, mt: int, limit: float = 0.0,
-             alpha: float = 0.0, tiles=None, src=None) -> None:
-    grouped = tiles is not None
-    groups, _, kb = _mx_check(rows, w, bias, grouped)
-    m = rows.shape[0] if src is None else src.numel()
-    _check(_LIB.vdamd_mx_gemm(_ptr(out), 0 if out is None else out.stride(0), _ptr(os), 0 if os is None else os.stride(0), _ptr(partial),
-                              rows.payload.data_ptr(), rows.payload.stride(0), rows.scales.data_ptr(), rows.scales.stride(0),
-                              rows.shape[0], w.qw.data_ptr(), w.ws.data_ptr(), _ptr(bias), m, w.rows, kb, ksplit, epi, float(limit),
-                              float(alpha), _ptr(tiles), 0 if tiles is None else tiles.shape[0], groups, _ptr(src), mt,
+def _mx_gemm(epi: int, rows: quant.MxRows, w: quant.MxWeight, groups: int, kb: int, bias, out, ldo: int, os, ldos: int, partial,
+             ksplit: int, mt: int, limit: float = 0.0, alpha: float = 0.0, tiles=None, src=None) -> None:
+    q, s = rows.payload, rows.scales
+    x_rows, ldq = q.shape
+    _check(_LIB.vdamd_mx_gemm(_ptr(out), ldo, _ptr(os), ldos, _ptr(partial), q.data_ptr(), ldq, s.data_ptr(), s.shape[1], x_rows,
+                              w.qw.data_ptr(), w.ws.data_ptr(), _ptr(bias), x_rows if src is None else src.numel(), w.rows, kb, ksplit, epi,
+                              limit, alpha, _ptr(tiles), 0 if tiles is None else tiles.shape[0], groups, _ptr(src), mt,
                               _DT[rows.dtype], _stream()), "mx_gemm")
 
 
 def mx_linear(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    _, _, kb = _mx_check(rows, w, bias, False)
-    m = rows.shape[0]
-    out = torch.empty((m, w.rows), dtype=rows.dtype, device=rows.device)
+    _, nt, kb = _mx_check(rows, w, bias, False)
+    m, n, dev = rows.payload.shape[0], w.rows, rows.payload.device
+    out = torch.empty((m, n), dtype=rows.dtype, device=dev)
     if m:
-        mt, ksplit = mx_plan(m, w.rows, kb, mx_big_ok(rows, w))
-        partial = torch.empty((ksplit, m, w.rows), dtype=torch.float32, device=rows.device) if ksplit > 1 else None
-        _mx_gemm(0, rows, w, bias, out, None, partial, ksplit, mt)
+        mt, ksplit = mx_plan(m, n, kb, mx_big_ok(m, nt, kb))
+        partial = torch.empty((ksplit, m, n), dtype=torch.float32, device=dev) if ksplit > 1 else None
+        _mx_gemm(0, rows, w, 1, kb, bias, out, n, None, 0, partial, ksplit, mt)
     return out
 
 
 def mx_linear_partials(rows: quant.MxRows, w: quant.MxWeight) -> Optional[torch.Tensor]:
     """``mx_linear`` left as fp32 slabs ``[ks, M, N]``; None where K is not split."""
-    _, _, kb = _mx_check(rows, w, None, False)
-    m = rows.shape[0]
-    mt, ksplit = mx_plan(m, w.rows, kb) if m else (1, 1)
+    _, nt, kb = _mx_check(rows, w, None, False)
+    m, n = rows.payload.shape[0], w.rows
+    mt, ksplit = mx_plan(m, n, kb, mx_big_ok(m, nt, kb)) if m else (1, 1)
     if ksplit == 1:
         return None
-    partial = torch.empty((ksplit, m, w.rows), dtype=torch.float32, device=rows.device)
-    _mx_gemm(1, rows, w, None, None, None, partial, ksplit, mt)
+    partial = torch.empty((ksplit, m, n), dtype=torch.float32, device=rows.payload.device)
+    _mx_gemm(1, rows, w, 1, kb, None, None, 0, None, 0, partial, ksplit, mt)
     return partial
 
 
 def _mx_gated_out(rows: quant.MxRows, w: quant.MxWeight, m: int) -> quant.MxRows:
     assert w.rows % 256 == 0, f"{w.rows} rows of gate and up: halves of whole 128 are wanted (pack_mx with halves=2)"
-    return quant.MxRows.empty(m, w.rows // 2, 8, rows.dtype, rows.device)
+    return quant.MxRows.empty(m, w.rows // 2, 8, rows.dtype, rows.payload.device)
 
 
 def mx_gate_up(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float, alpha: float) -> quant.MxRows:
-    m = rows.shape[0]
+    m = rows.payload.shape[0]
+    _, nt, kb = _mx_check(rows, w, bias, False)
     r = _mx_gated_out(rows, w, m)
-    _mx_check(rows, w, bias, False)
     if m:
-        _mx_gemm(2, rows, w, bias, r.payload, r.scales, None, 1, mx_plan(m, w.rows, 1, mx_big_ok(rows, w))[0], limit, alpha)
+        _mx_gemm(2, rows, w, 1, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None, 1,
+                 mx_plan(m, w.rows, 1, mx_big_ok(m, nt, kb))[0], limit, alpha)
     return r
 
 
@@ -2606,9 +2614,7 @@ def mx_sorted_ok(slots: int, w: quant.MxWeight) -> bool:
 
 def mx_sorted_rows(x, src_row: torch.Tensor) -> quant.MxRows:
     """``x[src_row]`` in 8 bits, ``x`` 16-bit rows or ``MxRows``."""
-    if not isinstance(x, quant.MxRows):
-        return mx_quantize(x, 8, src_row=src_row)
-    return quant.MxRows(x.payload.index_select(0, src_row), x.scales.index_select(0, src_row), x.width, x.bits, x.dtype)
+    return x.take(src_row) if isinstance(x, quant.MxRows) else mx_quantize(x, 8, src_row=src_row)
 
 
 def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], device: torch.device) -> int:
@@ -2616,7 +2622,7 @@ def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], 
     assert src is None or (src.dtype == torch.int32 and src.dim() == 1 and src.is_contiguous())
     assert tile_rows in (16, 32, 64, 256), tile_rows
     assert tile_rows < 256 or src is None, "tiles of 256 rows: the rows themselves, in order"
-    _mx_device(device, tiles, src)
+    _mx_device(device.index, tiles, src)
     return tile_rows // 16
 
 
@@ -2625,16 +2631,18 @@ def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor
     """Product of rows sorted by matrix (``moe_align``) with ``w``'s matrices; ``src_row``: the rows are ``rows[src_row]``.  Rows of no
     tile stay unwritten."""
     mt = _mx_tiles(tiles, tile_rows, src_row, rows.device)
+    groups, _, kb = _mx_check(rows, w, bias, True)
     out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=rows.dtype, device=rows.device)
     if out.shape[0]:
-        _mx_gemm(0, rows, w, bias, out, None, None, 1, mt, tiles=tiles, src=src_row)
+        _mx_gemm(0, rows, w, groups, kb, bias, out, w.rows, None, 0, None, 1, mt, tiles=tiles, src=src_row)
     return out
 
 
 def mx_grouped_gate_up(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor],
                        limit: float, alpha: float, src_row: Optional[torch.Tensor] = None) -> quant.MxRows:
     mt = _mx_tiles(tiles, tile_rows, src_row, rows.device)
+    groups, _, kb = _mx_check(rows, w, bias, True)
     r = _mx_gated_out(rows, w, rows.shape[0] if src_row is None else src_row.numel())
     if r.shape[0]:
-        _mx_gemm(2, rows, w, bias, r.payload, r.scales, None, 1, mt, limit, alpha, tiles, src_row)
+        _mx_gemm(2, rows, w, groups, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None, 1, mt, limit, alpha, tiles, src_row)
     return r

@@ -220,8 +220,8 @@ class MxRows:
     neighbours of a row; a scale byte of 255 makes its block NaN.
 
     ``q`` ``[M, K]`` float8_e4m3fn (8 bits) or ``[M, K/2]`` uint8 (4 bits, the even element in the low half of a byte), ``s``
-    ``[M, K/32]`` float8_e8m0fnu; ``dtype``: the type that products of these rows have.  Both are views of buffers whose rows are
-    padded (elements with zeros to a multiple of 128 columns, scales to 16 bytes), which is what the kernels read."""
+    ``[M, K/32]`` float8_e8m0fnu; ``dtype``: the type that products of these rows have.  Both are views of ``payload`` and ``scales``,
+    whose rows are padded (elements with zeros to a multiple of 128 columns, scales to 16 bytes), which is what the kernels read."""
     __slots__ = ("payload", "scales", "width", "bits", "dtype")
 
     def __init__(self, payload: torch.Tensor, scales: torch.Tensor, width: int, bits: int, dtype: torch.dtype):
@@ -230,13 +230,14 @@ class MxRows:
     @staticmethod
     def empty(rows: int, width: int, bits: int, dtype: torch.dtype, device) -> "MxRows":
         """Buffers for a kernel to fill (uninitialised)."""
-        if bits not in MX_LARGEST:
+        if bits != 8 and bits != 4:
             raise ValueError(f"microscaled rows hold 8 or 4 bits a value, not {bits}")
         if width <= 0 or width % MX_BLOCK:
             raise ValueError(f"{width} columns are not whole blocks of {MX_BLOCK}")
-        kp = _ceil_to(width, 128)
-        return MxRows(torch.empty((rows, kp * bits // 8), dtype=torch.uint8, device=device),
-                      torch.empty((rows, _ceil_to(kp // MX_BLOCK, 16)), dtype=torch.uint8, device=device), width, bits, dtype)
+        kp = (width + 127) // 128 * 128
+        payload = (torch.empty((rows, kp), dtype=torch.float8_e4m3fn, device=device) if bits == 8
+                   else torch.empty((rows, kp // 2), dtype=torch.uint8, device=device))
+        return MxRows(payload, torch.empty((rows, (kp + 511) // 512 * 16), dtype=torch.float8_e8m0fnu, device=device), width, bits, dtype)
 
     @staticmethod
     def of(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> "MxRows":
@@ -248,19 +249,26 @@ class MxRows:
         if q.dim() != 2 or s.dim() != 2 or width % MX_BLOCK or tuple(s.shape) != (q.shape[0], width // MX_BLOCK):
             raise ValueError(f"elements {tuple(q.shape)} and scales {tuple(s.shape)} are not rows of blocks of {MX_BLOCK}")
         r = MxRows.empty(q.shape[0], width, bits, dtype, q.device)
-        r.payload.zero_()
-        r.payload[:, :q.shape[1]] = q.view(torch.uint8)
-        r.scales[:, :s.shape[1]] = s.view(torch.uint8)
+        r.payload.view(torch.uint8).zero_()
+        r.payload.view(torch.uint8)[:, :q.shape[1]] = q.view(torch.uint8)
+        r.scales.view(torch.uint8).zero_()
+        r.scales.view(torch.uint8)[:, :s.shape[1]] = s.view(torch.uint8)
         return r
+
+    def take(self, rows: torch.Tensor) -> "MxRows":
+        """The rows of these numbers."""
+        return MxRows(self.payload.view(torch.uint8).index_select(0, rows).view(self.payload.dtype),
+                      self.scales.view(torch.uint8).index_select(0, rows).view(self.scales.dtype), self.width, self.bits, self.dtype)
 
     @property
     def q(self) -> torch.Tensor:
-        p = self.payload[:, :self.width * self.bits // 8]
-        return p.view(torch.float8_e4m3fn) if self.bits == 8 else p
+        n = self.width * self.bits // 8
+        return self.payload if self.payload.shape[1] == n else self.payload[:, :n]
 
     @property
     def s(self) -> torch.Tensor:
-        return self.scales[:, :self.width // MX_BLOCK].view(torch.float8_e8m0fnu)
+        n = self.width // MX_BLOCK
+        return self.scales if self.scales.shape[1] == n else self.scales[:, :n]
 
     @property
     def shape(self) -> Tuple[int, int]:
