@@ -29,6 +29,7 @@ struct MxArgs {
   float limit, alpha;               // MX_GLU: limit 0: SiLU
   // experts: row tiles (matrix, first row, rows) of rows sorted by expert; sorted row r is row src[r] of x (src null: r)
   const int* tiles; int num_tiles; int groups; const int* src; int x_rows;
+  const void* x16; long ldx; int K; // rows of the model type with K columns, quantised in the kernel (xq null)
 };
 
 __device__ __forceinline__ f32x4 mx_mfma(mx_u32x4 w, mx_i32x8 x, f32x4 c, uint32_t sw, uint32_t sx) {
@@ -79,13 +80,14 @@ __device__ __forceinline__ void mx_store_block(uint8_t* q, uint8_t* s, const flo
 #endif
 }
 
-// Few rows: the weights' bytes are the time.  A workgroup has four 16-column tiles (MX_GLU: two of the gate and the two of the same
-// columns of the up half); its four waves split K, each streaming its part of the tiles straight into registers; MT row tiles of x
-// come from the caches.  grid = (tiles / 4, ksplit, row tiles)
-constexpr int MX_NT = 4;
-template <typename T, int MT, int EPI>
-__global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
-  __shared__ f32x4 red[4][MX_NT][MT][64];
+// Few rows: the weights' bytes are the time.  A workgroup has NT 16-column tiles (MX_GLU: two of the gate and the two of the same columns
+// of the up half); its waves split K, each streaming its part of the tiles straight into registers, PF steps ahead; MT row tiles of x
+// come from the caches.  QUANT: x holds 16-bit rows, at most 16, which every workgroup quantises for itself into LDS while its first
+// weights are on their way: one launch instead of two.  grid = (tiles / NT, ksplit, row tiles)
+template <typename T, int MT, int NT, int WAVES, int EPI, bool QUANT, int PF>
+__global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(const MxArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];      // QUANT: rows of payload, 16 bytes apart from a multiple of 128; scales
+  __shared__ f32x4 red[WAVES][NT][MT][64];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int KB = a.KB, SS = (KB + 3) >> 2, ntiles = (a.N + 15) >> 4;
@@ -102,70 +104,127 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
   const uint8_t* ws = a.ws + (long)group * ntiles * SS * 256;
   const T* bias = a.bias == nullptr ? nullptr : (const T*)a.bias + (long)group * a.N;
 
-  int nt[MX_NT];
+  const uint8_t *wp[NT], *wsp[NT];
 #pragma unroll
-  for (int t = 0; t < MX_NT; ++t) {
-    if (EPI == MX_GLU) nt[t] = 2 * blockIdx.x + (t & 1) + (t >> 1) * (ntiles >> 1);
-    else nt[t] = min(4 * (int)blockIdx.x + t, ntiles - 1);
+  for (int t = 0; t < NT; ++t) {
+    const int nt = EPI == MX_GLU ? 2 * (int)blockIdx.x + (t & 1) + (t >> 1) * (ntiles >> 1) : min(NT * (int)blockIdx.x + t, ntiles - 1);
+    wp[t] = qw + (long)nt * KB * 1024 + lane * 16;
+    wsp[t] = ws + (long)nt * SS * 256 + lane * 4;
   }
+  // this workgroup's steps, this wave's
+  const int w_lo = (int)((long)KB * blockIdx.y / a.ksplit), w_n = (int)((long)KB * (blockIdx.y + 1) / a.ksplit) - w_lo;
+  const int lo = w_lo + w_n * wid / WAVES, hi = w_lo + w_n * (wid + 1) / WAVES;
+
   const uint8_t *xp[MT], *sp[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    long row = row0 + min(16 * i + r, rows - 1);
-    if (a.src != nullptr) row = min(max(a.src[row], 0), a.x_rows - 1);
-    xp[i] = a.xq + row * a.ldq + 16 * q;
-    sp[i] = a.xs + row * a.lds + q;
+    const int rr = min(16 * i + r, rows - 1);
+    if constexpr (QUANT) {
+      xp[i] = dyn + rr * (128 * w_n + 16) + 16 * q - 128 * w_lo;
+      sp[i] = dyn + rows * (128 * w_n + 16) + rr * (4 * w_n) + q - 4 * w_lo;
+    } else {
+      long row = row0 + rr;
+      if (a.src != nullptr) row = min(max(a.src[row], 0), a.x_rows - 1);
+      xp[i] = a.xq + row * a.ldq + 16 * q;
+      sp[i] = a.xs + row * a.lds + q;
+    }
   }
-  // this wave's steps
-  const int part = blockIdx.y * 4 + wid, parts = 4 * a.ksplit;
-  const int lo = (int)((long)KB * part / parts), hi = (int)((long)KB * (part + 1) / parts);
 
-  f32x4 acc[MX_NT][MT];
+  f32x4 acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < MX_NT; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  mx_u32x4 w[2][MX_NT];
-  mx_i32x8 x[2][MT];
-  uint32_t sw[2][MX_NT], sx[2][MT];
-  auto load = [&](int b, int k) {
+  mx_u32x4 w[PF][NT];
+  mx_i32x8 x[PF][MT];
+  uint32_t sw[PF][NT], sx[PF][MT];
+  auto load_w = [&](int b, int k) {
 #pragma unroll
-    for (int t = 0; t < MX_NT; ++t) {
-      w[b][t] = *reinterpret_cast<const mx_u32x4*>(qw + ((long)nt[t] * KB + k) * 1024 + lane * 16);
-      sw[b][t] = ws[((long)nt[t] * SS + (k >> 2)) * 256 + lane * 4 + (k & 3)];
+    for (int t = 0; t < NT; ++t) {
+      const mx_u32x4* const p = reinterpret_cast<const mx_u32x4*>(wp[t] + k * 1024L);
+      // One row tile reads a weight once: past the caches (51 experts of 3 x 2880 x 2880 83 + 43 -> 76 + 39 us, 2 x 28672 columns of 8192
+      // by 13 rows 53 -> 50)
+      if constexpr (MT == 1) w[b][t] = __builtin_nontemporal_load(p);
+      else w[b][t] = *p;
+      sw[b][t] = wsp[t][(k >> 2) * 256 + (k & 3)];
     }
+  };
+  auto load_x = [&](int b, int k) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      x[b][i] = mx_fragment(xp[i] + 128L * k, xp[i] + 128L * k + 64);
+      x[b][i] = mx_fragment(xp[i] + 128 * k, xp[i] + 128 * k + 64);
       sx[b][i] = sp[i][4 * k];
     }
   };
-  auto mma = [&](int b) {
 #pragma unroll
-    for (int t = 0; t < MX_NT; ++t)
+  for (int u = 0; u < PF; ++u)
+    if (lo + u < hi) {
+      load_w(u, lo + u);
+      if constexpr (!QUANT) load_x(u, lo + u);
+    }
+  if constexpr (QUANT) {
+    const T* src = (const T*)a.x16;
+    uint8_t* const scales = dyn + rows * (128 * w_n + 16);
+    const int vecs = 16 * w_n;                                   // of 8 values, in a row's part (columns from K on are zeros)
+    for (int i = threadIdx.x; i < rows * vecs; i += 64 * WAVES) {
+      const int m = i / vecs, c = i - m * vecs, k = 128 * w_lo + 8 * c;
+      float v[8];
+      if (k < a.K) {
+        mx_load8(src + (long)(row0 + m) * a.ldx + k, v);
+      } else {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[t][i] = mx_mfma(w[b][t], x[b][i], acc[t][i], sw[b][t], sx[b][i]);
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      }
+      mx_store8(dyn + m * (128 * w_n + 16) + 8 * c, scales + m * (4 * w_n) + (c >> 2), v);
+    }
+    __syncthreads();
+  }
+  auto mma = [&](int u, int k) {
+    if constexpr (QUANT) load_x(u, k);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[t][i] = mx_mfma(w[u][t], x[u][i], acc[t][i], sw[u][t], sx[u][i]);
   };
-  if (lo < hi) load(0, lo);
-  for (int k = lo; k < hi; k += 2) {
-    if (k + 1 < hi) load(1, k + 1);
-    mma(0);
-    if (k + 1 < hi) {
-      if (k + 2 < hi) load(0, k + 2);
-      mma(1);
+  auto load = [&](int u, int k) {
+    load_w(u, k);
+    if constexpr (!QUANT) load_x(u, k);
+  };
+  int k = lo;
+  // (loads under a condition are waited for as if none had been issued behind them: only the last steps have any)
+  for (; k + 2 * PF <= hi; k += PF) {
+#pragma unroll
+    for (int u = 0; u < PF; ++u) {
+      mma(u, k + u);
+      load(u, k + u + PF);
     }
   }
+#pragma unroll
+  for (int u = 0; u < PF; ++u)
+    if (k + u < hi) {
+      mma(u, k + u);
+      if (k + u + PF < hi) load(u, k + u + PF);
+    }
+  k += PF;
+#pragma unroll
+  for (int u = 0; u < PF; ++u)
+    if (k + u < hi) mma(u, k + u);
 
 #pragma unroll
-  for (int t = 0; t < MX_NT; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < MT; ++i) red[wid][t][i][lane] = acc[t][i];
   __syncthreads();
-  auto sum = [&](int t, int i) { return (red[0][t][i][lane] + red[1][t][i][lane]) + (red[2][t][i][lane] + red[3][t][i][lane]); };
+  auto sum = [&](int t, int i) {
+    f32x4 v = red[0][t][i][lane];
+#pragma unroll
+    for (int p = 1; p < WAVES; ++p) v += red[p][t][i][lane];
+    return v;
+  };
   if constexpr (EPI == MX_GLU) {
     const int cols = a.N >> 1, n = 32 * blockIdx.x + 4 * q;
-    for (int i = wid; i < MT; i += 4) {
+    for (int i = wid; i < MT; i += WAVES) {
       const int m = 16 * i + r;
       float v[2][4];
 #pragma unroll
@@ -181,13 +240,11 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(const MxArgs a) {
       mx_store_block((uint8_t*)a.out + row * a.ldo + 32 * blockIdx.x, a.os + row * a.ldos + blockIdx.x, v, lane, m < rows);
     }
   } else {
-    const int tile = 4 * blockIdx.x + wid, n = 16 * tile + 4 * q;
-    if (n >= a.N) return;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = 16 * i + r;
-      const f32x4 v = sum(wid, i);
-      if (m >= rows) continue;
+    for (int j = wid; j < NT * MT; j += WAVES) {
+      const int t = j % NT, i = j / NT;
+      const int n = 16 * (NT * (int)blockIdx.x + t) + 4 * q, m = 16 * i + r;
+      if (n >= a.N || m >= rows) continue;
+      const f32x4 v = sum(t, i);
       if constexpr (EPI == MX_SLAB) {
         *reinterpret_cast<f32x4*>(a.partial + ((long)blockIdx.y * a.M + row0 + m) * a.N + n) = v;
       } else {
@@ -551,64 +608,93 @@ __global__ __launch_bounds__(256) void mx_reduce_kernel(T* __restrict__ out, lon
   *reinterpret_cast<typename Vec4<T>::type*>(out + m * ldo + n) = o;
 }
 
+// shapes of a launch of the streaming kernel: one row tile with 1 or 2 column tiles and 8 waves (not MX_GLU) or 4 and 8, and with 4 column
+// tiles and 4 waves 1, 2 or 4 row tiles
 template <typename T, int EPI>
-int mx_stream(const MxArgs& a, int mt, hipStream_t st) {
+int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
   const int ntiles = (a.N + 15) / 16;
-  dim3 grid((ntiles + 3) / 4, a.ksplit, a.tiles != nullptr ? a.num_tiles : (a.M + 16 * mt - 1) / (16 * mt));
+  dim3 grid((ntiles + nt - 1) / nt, a.ksplit, a.tiles != nullptr ? a.num_tiles : (a.M + 16 * mt - 1) / (16 * mt));
   if (grid.y > 65535 || grid.z > 65535) return -7;
-  switch (mt) {
-    case 1: mx_stream_kernel<T, 1, EPI><<<grid, 256, 0, st>>>(a); break;
-    case 2: mx_stream_kernel<T, 2, EPI><<<grid, 256, 0, st>>>(a); break;
-    case 4: mx_stream_kernel<T, 4, EPI><<<grid, 256, 0, st>>>(a); break;
-    default: return -6;
+#define GO(M_, N_, W_, Q_, P_) mx_stream_kernel<T, M_, N_, W_, EPI, Q_, P_><<<grid, 64 * W_, lds, st>>>(a)
+  size_t lds = 0;
+  const bool quant = a.x16 != nullptr;
+  if (quant) {
+    lds = (size_t)a.M * (132 * ((a.KB + a.ksplit - 1) / a.ksplit) + 16);
+    if (mt != 1 || a.M > 16 || lds > 49152 || a.tiles != nullptr) return -6;
   }
+  if (nt == 4 && waves == 4) {
+    if (quant) GO(1, 4, 4, true, 3);
+    else if (mt == 1) GO(1, 4, 4, false, 3);
+    else if (mt == 2) GO(2, 4, 4, false, 2);
+    else if (mt == 4) GO(4, 4, 4, false, 2);
+    else return -6;
+  } else if (nt == 4 && waves == 8 && mt == 1) {
+    if (quant) GO(1, 4, 8, true, 3);
+    else GO(1, 4, 8, false, 3);
+  } else if constexpr (EPI != MX_GLU) {
+    if (mt != 1 || waves != 8 || (nt != 1 && nt != 2)) return -6;
+    if (nt == 1 && quant) GO(1, 1, 8, true, 6);
+    else if (nt == 1) GO(1, 1, 8, false, 6);
+    else if (quant) GO(1, 2, 8, true, 4);
+    else GO(1, 2, 8, false, 4);
+  } else {
+    return -6;
+  }
+#undef GO
   HIP_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename T>
-int mx_dispatch(const MxArgs& a, int epi, int mt, hipStream_t st) {
+int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t st) {
   if (mt == 16) {
-    if (a.ksplit != 1 || a.src != nullptr) return -1;
+    if (a.ksplit != 1 || a.src != nullptr || a.x16 != nullptr) return -1;
     return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : -1;
   }
-  if (epi == MX_GLU) return mx_stream<T, MX_GLU>(a, mt, st);
+  if (epi == MX_GLU) return mx_stream<T, MX_GLU>(a, mt, nt, waves, st);
   if (epi == MX_SLAB || a.ksplit > 1) {
-    const int rc = mx_stream<T, MX_SLAB>(a, mt, st);
+    const int rc = mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
     if (rc != 0 || epi == MX_SLAB) return rc;
     const long n = (long)a.M * (a.N / 4);
     mx_reduce_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>((T*)a.out, a.ldo, a.partial, (const T*)a.bias, a.M, a.N, a.ksplit);
     HIP_LAUNCH_CHECK();
     return 0;
   }
-  return mx_stream<T, MX_OUT>(a, mt, st);
+  return mx_stream<T, MX_OUT>(a, mt, nt, waves, st);
 }
 
 }  // namespace
 
 // xq [x_rows][128 KB] bytes (rows ldq apart, a multiple of 128), xs [x_rows][4 KB] scale bytes (rows lds apart, a multiple of 4); qw, ws as
 // above for `groups` matrices of N rows (padded to 16), N % 8 == 0.
+// Or xq null: x16, rows of K columns of the model type (ldx elements apart, a multiple of 8), K % 32 == 0, at most 128 KB, quantised
+// inside: at most 16 rows, of which a workgroup's part fits 48 KiB; no tiles.
 // epi 0: out [M][N] of the model type, rows ldo elements apart (ksplit > 1: through partial [ksplit][M][N]); 1: partial alone;
 // 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales, ksplit 1; limit 0: SiLU.
-// tiles [num_tiles][3] (matrix, first row, rows) or null; src [M] or null: the row of x behind each row.  row_tiles: 16-row tiles a
-// workgroup takes (1, 2 or 4; of `tiles` at most 16 row_tiles rows each); 16: the kernel of 256-row tiles (ksplit 1, src null, x_rows ldq
-// and a matrix's bytes below 2^32, lds a multiple of 16).
+// tiles [num_tiles][3] (matrix, first row, rows) or null; src [M] or null: the row of x behind each row.  shape: 16-row tiles a
+// workgroup takes (1, 2 or 4; of `tiles` at most 16 times as many rows each) + 256 times its 16-column tiles + 65536 times its waves;
+// 16: the kernel of 256-row tiles (ksplit 1, src null, x_rows ldq and a matrix's bytes below 2^32, lds a multiple of 16).
 VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* partial, const void* xq, long ldq, const void* xs, long lds,
-                            int x_rows, const void* qw, const void* ws, const void* bias, int M, int N, int KB, int ksplit, int epi,
-                            float limit, float alpha, const int* tiles, int num_tiles, int groups, const int* src, int row_tiles,
-                            int dtype, void* stream) {
+                            int x_rows, const void* x16, long ldx, int K, const void* qw, const void* ws, const void* bias, int M, int N,
+                            int KB, int ksplit, int epi, float limit, float alpha, const int* tiles, int num_tiles, int groups,
+                            const int* src, int shape, int dtype, void* stream) {
   if (M <= 0 || (tiles != nullptr && num_tiles <= 0)) return 0;
-  if (N <= 0 || N % 8 || KB <= 0 || x_rows <= 0 || groups <= 0 || ksplit < 1 || ksplit > KB || (src == nullptr && x_rows < M)) return -1;
-  if (ldq % 128 || ldq < 128L * KB || lds < 4L * KB || ((uintptr_t)xq | (uintptr_t)qw) % 16 || ((uintptr_t)ws | (uintptr_t)bias) % 4) return -1;
+  if (N <= 0 || N % 8 || KB <= 0 || groups <= 0 || ksplit < 1 || ksplit > KB) return -1;
+  if (((uintptr_t)qw % 16) || ((uintptr_t)ws | (uintptr_t)bias) % 4) return -1;
+  if (x16 != nullptr) {
+    if (K <= 0 || K % 32 || K > 128L * KB || ldx % 8 || ldx < K || (uintptr_t)x16 % 16 || src != nullptr) return -1;
+  } else if (x_rows <= 0 || (src == nullptr && x_rows < M) || ldq % 128 || ldq < 128L * KB || lds < 4L * KB || (uintptr_t)xq % 16) {
+    return -1;
+  }
   if (epi == MX_GLU && (N % 256 || ksplit != 1 || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
   if (epi == MX_OUT && (ldo % 8 || ldo < N || (uintptr_t)out % 16 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;
   if ((ksplit > 1 || epi == MX_SLAB) && tiles != nullptr) return -1;
   if (epi < 0 || epi > 2) return -1;
   const MxArgs a = {(const uint8_t*)xq, ldq, (const uint8_t*)xs, lds, (const uint8_t*)qw, (const uint8_t*)ws, out, ldo, (uint8_t*)os, ldos,
-                    partial, bias, M, N, KB, ksplit, limit, alpha, tiles, num_tiles, groups, src, x_rows};
+                    partial, bias, M, N, KB, ksplit, limit, alpha, tiles, num_tiles, groups, src, x_rows, x16, ldx, K};
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_BF16) return mx_dispatch<bf16_t>(a, epi, row_tiles, st);
-  if (dtype == DT_F16) return mx_dispatch<f16_t>(a, epi, row_tiles, st);
+  if (dtype == DT_BF16) return mx_dispatch<bf16_t>(a, epi, shape & 255, shape >> 8 & 255, shape >> 16, st);
+  if (dtype == DT_F16) return mx_dispatch<f16_t>(a, epi, shape & 255, shape >> 8 & 255, shape >> 16, st);
   return -2;
 }

@@ -242,7 +242,7 @@ def test_linear_rows_do_not_mix(m):
     assert y[:, 37].isnan().all() and torch.equal(y[:, cols.cuda()], clean[:, cols.cuda()])
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 512, 4096), (64, 2880, 4096)])
+@pytest.mark.parametrize("m,n,k", [(40, 512, 4096), (64, 2880, 4096)])
 def test_partials_and_the_norm_behind_them(m, n, k):
     from vllm_distributed_amd import ops
     x, residual, gain = rows(m, k), rows(m, n), (1 + 0.1 * torch.randn(n)).to(torch.bfloat16)

@@ -543,34 +543,43 @@ def reduce_add_rms_norm_mx(partial, residual, weight, eps) -> Tuple[MxRows, torc
     return torch_ref.rms_norm_mx(partial.sum(0), residual, weight, eps)
 
 
-def _mx_operand(x, w: MxWeight) -> MxRows:
-    """``x`` (16-bit rows, quantised here, or rows that are 8-bit already) as the left operand of a product with ``w``."""
-    rows = x if isinstance(x, MxRows) else mx_quantize(x, 8)
-    if rows.bits != 8:
-        raise ValueError("products take 8-bit microscaled rows")
-    if (rows.width + 127) // 128 != w.qw.shape[-3]:
-        raise ValueError(f"rows of {rows.width} columns and a weight of {w.qw.shape[-3] * 128} (padded)")
-    return rows
+def _mx_operand(x, w: MxWeight):
+    """``x`` as the left operand of a product with ``w``: ``MxRows``, or on the GPU a few 16-bit rows that the product quantises itself."""
+    if isinstance(x, MxRows):
+        if x.bits != 8:
+            raise ValueError("products take 8-bit microscaled rows")
+        width = x.width
+    else:
+        width = x.shape[-1]
+        _mx_width(width)
+    kb = w.qw.shape[-3]
+    if (width + 127) // 128 != kb:
+        raise ValueError(f"rows of {width} columns and a weight of {kb * 128} (padded)")
+    if isinstance(x, MxRows):
+        return x
+    return _hip.mx_operand(x, kb) if _mx_hip(x, x.dtype) else mx_quantize(x, 8)
+
+
+def _mx_on_gpu(x) -> bool:
+    return _mx_hip(x.payload if isinstance(x, MxRows) else x, x.dtype)
 
 
 def mx_linear(x, weight: MxWeight, bias=None):
     """``y = x W^T (+ bias)`` for a 4-bit microscaled weight (``ops.quant.pack_mx``) and rows in 8 bits (``x``: an ``MxRows``, or 16-bit
     rows that are quantised here), on the scaled matrix instructions with 32-bit sums."""
     rows = _mx_operand(x, weight)
-    if _mx_hip(rows.payload, rows.dtype):
-        y = _hip.mx_linear(rows, weight, bias)
-    else:
-        y = quant.mx_product(rows, weight, bias).to(rows.dtype)
-    return y if isinstance(x, MxRows) else y.view(x.shape[:-1] + (y.shape[-1],))
+    y = _hip.mx_linear(rows, weight, bias) if _mx_on_gpu(rows) else quant.mx_product(rows, weight, bias).to(rows.dtype)
+    return y if isinstance(x, MxRows) or x.dim() == 2 else y.view(x.shape[:-1] + (y.shape[-1],))
 
 
 def mx_linear_partials(x, weight: MxWeight):
     """``mx_linear`` without a bias left as fp32 K-split slabs ``[ks, M, N]`` for the norm or the rotary kernel that follows; None where
     the product runs unsplit."""
-    if not (_use_hip(x.payload if isinstance(x, MxRows) else x) and envs.VDAMD_FUSED_REDUCE_NORM):
+    if not (_mx_on_gpu(x) and envs.VDAMD_FUSED_REDUCE_NORM):
         return None
-    rows = _mx_operand(x, weight)
-    return _hip.mx_linear_partials(rows, weight) if rows.dtype in (torch.bfloat16, torch.float16) else None
+    if not _hip.mx_splits(x.shape[0], weight):
+        return None
+    return _hip.mx_linear_partials(_mx_operand(x, weight), weight)
 
 
 def mx_gate_up(x, weight: MxWeight, bias=None, limit: float = 0.0, alpha: float = 1.702) -> MxRows:
@@ -580,7 +589,7 @@ def mx_gate_up(x, weight: MxWeight, bias=None, limit: float = 0.0, alpha: float 
     rows = _mx_operand(x, weight)
     if weight.rows % 256:
         raise ValueError(f"{weight.rows} rows of gate and up: halves of whole 128 are wanted (pack_mx with halves=2)")
-    if _mx_hip(rows.payload, rows.dtype):
+    if _mx_on_gpu(rows):
         return _hip.mx_gate_up(rows, weight, bias, limit, alpha)
     return quant.mx_quantize(quant.mx_gated(quant.mx_product(rows, weight, bias), limit, alpha), 8, rows.dtype)
 
@@ -594,6 +603,9 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
     e_local = weight13.qw.shape[0]
     total = num_experts or (e_local if local_experts < 0 else expert_start + local_experts)
     t, k = topi.shape
+    width = x.width if isinstance(x, MxRows) else x.shape[-1]
+    if (width + 127) // 128 != weight13.qw.shape[-3] or width % 32:
+        raise ValueError(f"rows of {width} columns and experts of {weight13.qw.shape[-3] * 128} (padded)")
     if len(x.shape) != 2 or x.shape[0] != t or topw.shape != topi.shape:
         raise ValueError(f"rows {tuple(x.shape)}, choices {tuple(topi.shape)}, weights {tuple(topw.shape)}")
     dtype = x.dtype
@@ -610,7 +622,7 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
             rows, src_row = _hip.mx_sorted_rows(x, src_row), None
         else:
             rows = x if isinstance(x, MxRows) else _hip.mx_quantize(x, 8)
-        a = _hip.mx_grouped_gate_up(_mx_operand(rows, weight13), weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
+        a = _hip.mx_grouped_gate_up(rows, weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
         y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2)
         return moe_combine(y, topw, topi, inv, expert_start, local_experts)
     return torch_ref.mx_experts(_mx_operand(x, weight13), topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)

@@ -99,7 +99,7 @@ def load() -> ctypes.CDLL:
         "vdamd_mx_quantize": [P, L, P, L, P, L, L, I, I, I, P, I, I, P],
         "vdamd_mx_dequantize": [P, P, L, P, L, L, I, I, I, P],
         "vdamd_mx_rms_norm": [P, L, P, L, P, P, L, P, I, P, P, F, I, I, I, I, P],
-        "vdamd_mx_gemm": [P, L, P, L, P, P, L, P, L, I, P, P, P, I, I, I, I, I, F, F, P, I, I, P, I, I, P],
+        "vdamd_mx_gemm": [P, L, P, L, P, P, L, P, L, I, P, L, I, P, P, P, I, I, I, I, I, F, F, P, I, I, P, I, I, P],
         "vdamd_layer_norm_to": [P, P, L, P, L, P, P, F, I, I, I, I, I, P],
         "vdamd_gated_rms_norm": [P, L, P, P, P, L, F, I, I, I, F, I, I, I, P],
         "vdamd_clamped_glu": [P, P, L, I, I, F, F, I, P],
@@ -2513,24 +2513,30 @@ def mx_rms_norm(x: Optional[torch.Tensor], slabs: Optional[torch.Tensor], residu
     return r, out
 
 
-def _mx_check(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor], grouped: bool) -> Tuple[int, int, int]:
-    """(matrices, 16-row tiles of each, 128-column steps) of a weight that ``rows`` can be multiplied with."""
+def _mx_check(x, w: quant.MxWeight, bias: Optional[torch.Tensor], grouped: bool) -> Tuple[int, int, int]:
+    """(matrices, 16-row tiles of each, 128-column steps) of a weight that ``x`` - ``MxRows``, or rows as ``_mx_rows`` leaves them - can
+    be multiplied with."""
     qw, ws, n = w
-    q, s, dtype = rows.payload, rows.scales, rows.dtype
-    assert rows.bits == 8 and (dtype == torch.bfloat16 or dtype == torch.float16), (rows.bits, dtype)
+    dtype = x.dtype
     shape = qw.shape
     assert len(shape) == (5 if grouped else 4) and shape[-1] == 4 and shape[-2] == 64 and qw.dtype == torch.int32 and qw.is_contiguous()
     nt, kb = shape[-4], shape[-3]
     assert ws.shape == (*shape[:-4], nt, (kb + 3) // 4, 64, 4) and ws.dtype == torch.uint8 and ws.is_contiguous(), (ws.shape, shape)
     assert n > 0 and n % 8 == 0 and nt == (n + 15) // 16, (n, nt)
-    m = q.shape[0]
-    assert q.shape[1] == 128 * kb, f"rows of {rows.width} columns, a weight of {128 * kb} with padding"
-    assert q.is_contiguous() and s.is_contiguous() and s.shape == (m, (kb + 3) // 4 * 16), (q.shape, s.shape)
+    assert dtype == torch.bfloat16 or dtype == torch.float16, dtype
+    if isinstance(x, quant.MxRows):
+        q, s = x.payload, x.scales
+        assert x.bits == 8 and q.shape[1] == 128 * kb, f"{x.bits}-bit rows of {x.width} columns, a weight of {128 * kb} with padding"
+        assert q.is_contiguous() and s.is_contiguous() and s.shape == (q.shape[0], (kb + 3) // 4 * 16), (q.shape, s.shape)
+        dev = q.get_device()
+    else:
+        s, dev = None, x.get_device()
+        assert x.shape[1] % 32 == 0 and (x.shape[1] + 127) // 128 == kb, (x.shape, kb)
     groups = shape[0] if grouped else 1
     if bias is not None:
         assert bias.dtype == dtype and bias.is_contiguous() and bias.data_ptr() % 4 == 0, (bias.dtype, dtype)
         assert bias.shape == ((groups, n) if grouped else (n,)), (bias.shape, groups, n)
-    _mx_device(q.get_device(), s, qw, ws, bias)
+    _mx_device(dev, s, qw, ws, bias)
     return groups, nt, kb
 
 
@@ -2543,60 +2549,98 @@ def mx_big_ok(m: int, nt: int, kb: int) -> bool:
     return m * kb * 128 < lim and nt * kb * 1024 < lim
 
 
-def mx_plan(m: int, n: int, kb: int, big: bool = False) -> Tuple[int, int]:
-    """(16-row tiles a workgroup takes, K split); ``big``: the kernel of 256-row tiles may be chosen."""
+MX_FUSED_BYTES = 49152             # of a workgroup's part of 16-bit rows that a product quantises itself
+MX_FUSED_ROWS = 4                  # (us, quantised apart / inside: 1 row of 4096 into 2880 columns 6.6 / 4.4, 4 into 28672 18.0 / 17.6, 8 18.2 / 21.6)
+
+
+def _mx_shape(mt: int, nt: int, waves: int) -> int:
+    return mt + 256 * nt + 65536 * waves
+
+
+def mx_plan(m: int, n: int, kb: int, big: bool, gated: bool = False) -> Tuple[int, int]:
+    """(shape of the launch, K split) of ``m`` rows against ``n`` columns; ``big``: the kernel of 256-row tiles may be chosen."""
     if big and m > 512:
         return MX_BIG, 1
-    mt = 1 if m <= 16 else 2 if m <= 32 else 4
+    tiles = (n + 15) // 16
+    if m <= 16:
+        # Column tiles a workgroup takes: more read x less often, fewer spread over the chip.  us with 1, 2 and 4: one row of 4096 into
+        # 6144 columns 5.5, 5.6, 6.6; of 28672 into 8192 20.7, 20.2, 23.9; 13 rows of 8192 into 8192 15.4, 11.2, 13.7; 16 of 8192 into
+        # 10240 22.3, 18.9, 15.4; 4 of 4096 into 28672 18.4, 15.8, 14.9; 8 of 8192 into 1280 7.6, 8.7, 10.4
+        nt = 4 if gated or tiles >= (640 if m > 4 else 1536) else 2 if tiles >= (256 if m > 4 else 448) else 1
+        return _mx_shape(1, nt, 4 if nt == 4 and tiles >= 1024 else 8), 1
+    mt = 2 if m <= 32 else 4
+    if gated:
+        return _mx_shape(mt, 4, 4), 1
     wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
-    return mt, max(1, min((512 + wgs - 1) // wgs, kb // 8))
+    return _mx_shape(mt, 4, 4), max(1, min((512 + wgs - 1) // wgs, kb // 8))
 
 
-def _mx_gemm(epi: int, rows: quant.MxRows, w: quant.MxWeight, groups: int, kb: int, bias, out, ldo: int, os, ldos: int, partial,
-             ksplit: int, mt: int, limit: float = 0.0, alpha: float = 0.0, tiles=None, src=None) -> None:
-    q, s = rows.payload, rows.scales
-    x_rows, ldq = q.shape
-    _check(_LIB.vdamd_mx_gemm(_ptr(out), ldo, _ptr(os), ldos, _ptr(partial), q.data_ptr(), ldq, s.data_ptr(), s.shape[1], x_rows,
-                              w.qw.data_ptr(), w.ws.data_ptr(), _ptr(bias), x_rows if src is None else src.numel(), w.rows, kb, ksplit, epi,
-                              limit, alpha, _ptr(tiles), 0 if tiles is None else tiles.shape[0], groups, _ptr(src), mt,
-                              _DT[rows.dtype], _stream()), "mx_gemm")
+def mx_fused_ok(m: int, kb: int) -> bool:
+    """Whether a product quantises ``m`` 16-bit rows of ``kb`` steps itself."""
+    return 0 < m <= MX_FUSED_ROWS and m * (132 * kb + 16) <= MX_FUSED_BYTES
 
 
-def mx_linear(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    _, nt, kb = _mx_check(rows, w, bias, False)
-    m, n, dev = rows.payload.shape[0], w.rows, rows.payload.device
-    out = torch.empty((m, n), dtype=rows.dtype, device=dev)
+def _mx_gemm(epi: int, x, w: quant.MxWeight, groups: int, kb: int, bias, out, ldo: int, os, ldos: int, partial, plan: Tuple[int, int],
+             limit: float = 0.0, alpha: float = 0.0, tiles=None, src=None) -> None:
+    """``x``: ``MxRows``, or 16-bit rows (``mx_fused_ok``)."""
+    if isinstance(x, quant.MxRows):
+        q, s = x.payload, x.scales
+        rows, ldq = q.shape
+        left = (q.data_ptr(), ldq, s.data_ptr(), s.shape[1], rows, None, 0, 0)
+    else:
+        rows, k = x.shape
+        left = (None, 0, None, 0, 0, x.data_ptr(), x.stride(0), k)
+    _check(_LIB.vdamd_mx_gemm(_ptr(out), ldo, _ptr(os), ldos, _ptr(partial), *left, w.qw.data_ptr(), w.ws.data_ptr(), _ptr(bias),
+                              rows if src is None else src.numel(), w.rows, kb, plan[1], epi, limit, alpha, _ptr(tiles),
+                              0 if tiles is None else tiles.shape[0], groups, _ptr(src), plan[0], _DT[x.dtype], _stream()), "mx_gemm")
+
+
+def mx_operand(x: torch.Tensor, kb: int):
+    """16-bit rows as the left operand of a product of ``kb`` steps: a few as they are, others quantised."""
+    return _mx_rows(x) if mx_fused_ok(x.numel() // x.shape[-1], kb) else mx_quantize(x, 8)
+
+
+def mx_linear(x, w: quant.MxWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _, nt, kb = _mx_check(x, w, bias, False)
+    m, n, dev = x.shape[0], w.rows, x.device
+    out = torch.empty((m, n), dtype=x.dtype, device=dev)
     if m:
-        mt, ksplit = mx_plan(m, n, kb, mx_big_ok(m, nt, kb))
-        partial = torch.empty((ksplit, m, n), dtype=torch.float32, device=dev) if ksplit > 1 else None
-        _mx_gemm(0, rows, w, 1, kb, bias, out, n, None, 0, partial, ksplit, mt)
+        plan = mx_plan(m, n, kb, mx_big_ok(m, nt, kb))
+        partial = torch.empty((plan[1], m, n), dtype=torch.float32, device=dev) if plan[1] > 1 else None
+        _mx_gemm(0, x, w, 1, kb, bias, out, n, None, 0, partial, plan)
     return out
 
 
-def mx_linear_partials(rows: quant.MxRows, w: quant.MxWeight) -> Optional[torch.Tensor]:
+def mx_splits(m: int, w: quant.MxWeight) -> bool:
+    """Whether a product of ``m`` rows runs with a split K."""
+    nt, kb = w.qw.shape[-4:-2]
+    return m > 0 and mx_plan(m, w.rows, kb, mx_big_ok(m, nt, kb))[1] > 1
+
+
+def mx_linear_partials(x, w: quant.MxWeight) -> Optional[torch.Tensor]:
     """``mx_linear`` left as fp32 slabs ``[ks, M, N]``; None where K is not split."""
-    _, nt, kb = _mx_check(rows, w, None, False)
-    m, n = rows.payload.shape[0], w.rows
-    mt, ksplit = mx_plan(m, n, kb, mx_big_ok(m, nt, kb)) if m else (1, 1)
-    if ksplit == 1:
+    _, nt, kb = _mx_check(x, w, None, False)
+    m, n = x.shape[0], w.rows
+    plan = mx_plan(m, n, kb, mx_big_ok(m, nt, kb)) if m else (0, 1)
+    if plan[1] == 1:
         return None
-    partial = torch.empty((ksplit, m, n), dtype=torch.float32, device=rows.payload.device)
-    _mx_gemm(1, rows, w, 1, kb, None, None, 0, None, 0, partial, ksplit, mt)
+    partial = torch.empty((plan[1], m, n), dtype=torch.float32, device=x.device)
+    _mx_gemm(1, x, w, 1, kb, None, None, 0, None, 0, partial, plan)
     return partial
 
 
-def _mx_gated_out(rows: quant.MxRows, w: quant.MxWeight, m: int) -> quant.MxRows:
+def _mx_gated_out(x, w: quant.MxWeight, m: int) -> quant.MxRows:
     assert w.rows % 256 == 0, f"{w.rows} rows of gate and up: halves of whole 128 are wanted (pack_mx with halves=2)"
-    return quant.MxRows.empty(m, w.rows // 2, 8, rows.dtype, rows.payload.device)
+    return quant.MxRows.empty(m, w.rows // 2, 8, x.dtype, x.device)
 
 
-def mx_gate_up(rows: quant.MxRows, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float, alpha: float) -> quant.MxRows:
-    m = rows.payload.shape[0]
-    _, nt, kb = _mx_check(rows, w, bias, False)
-    r = _mx_gated_out(rows, w, m)
+def mx_gate_up(x, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float, alpha: float) -> quant.MxRows:
+    m = x.shape[0]
+    _, nt, kb = _mx_check(x, w, bias, False)
+    r = _mx_gated_out(x, w, m)
     if m:
-        _mx_gemm(2, rows, w, 1, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None, 1,
-                 mx_plan(m, w.rows, 1, mx_big_ok(m, nt, kb))[0], limit, alpha)
+        _mx_gemm(2, x, w, 1, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None,
+                 mx_plan(m, w.rows, kb, mx_big_ok(m, nt, kb), True), limit, alpha)
     return r
 
 
@@ -2623,7 +2667,7 @@ def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], 
     assert tile_rows in (16, 32, 64, 256), tile_rows
     assert tile_rows < 256 or src is None, "tiles of 256 rows: the rows themselves, in order"
     _mx_device(device.index, tiles, src)
-    return tile_rows // 16
+    return MX_BIG if tile_rows == 256 else _mx_shape(tile_rows // 16, 4, 4)
 
 
 def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor] = None,
@@ -2634,7 +2678,7 @@ def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor
     groups, _, kb = _mx_check(rows, w, bias, True)
     out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=rows.dtype, device=rows.device)
     if out.shape[0]:
-        _mx_gemm(0, rows, w, groups, kb, bias, out, w.rows, None, 0, None, 1, mt, tiles=tiles, src=src_row)
+        _mx_gemm(0, rows, w, groups, kb, bias, out, w.rows, None, 0, None, (mt, 1), tiles=tiles, src=src_row)
     return out
 
 
@@ -2644,5 +2688,6 @@ def mx_grouped_gate_up(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tenso
     groups, _, kb = _mx_check(rows, w, bias, True)
     r = _mx_gated_out(rows, w, rows.shape[0] if src_row is None else src_row.numel())
     if r.shape[0]:
-        _mx_gemm(2, rows, w, groups, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None, 1, mt, limit, alpha, tiles, src_row)
+        _mx_gemm(2, rows, w, groups, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None, (mt, 1), limit, alpha, tiles,
+                 src_row)
     return r
