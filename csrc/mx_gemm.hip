@@ -592,6 +592,187 @@ int mx_big(const MxArgs& a, hipStream_t st) {
   return 0;
 }
 
+// Between: rows enough that x is worth sharing, too few to fill the chip with 256-row tiles.  A workgroup has 16 MT rows and 4 NT column
+// tiles, its four waves NT of them each and all of the rows; K in steps of 128, split over the grid.  x and the weights of S steps are in
+// LDS or on their way to it, straight from memory: the loads of the step that is S - 1 ahead go out while one is multiplied, so
+// (S - 1) (2 MT + 4 NT) KiB a workgroup are in flight, and the bytes of the weights are the time until the matrix cores are.
+// A step is one barrier: behind it every wave's loads of the step are there and every wave has read the step before.
+// Scales come 16 bytes a row (four steps) at a time, with the first step of each four, into sets of their own.
+// MX_GLU: NT 4, a wave's tiles are two of the gate and the same two of the up half - a block of 32 columns.
+template <int MT, int NT> struct MxRing {
+  static constexpr int X = MT * 2048, STEP = X + NT * 4096;               // bytes of a step
+  static constexpr int XR = MT < 4 ? 64 : 16 * MT, SCALES = XR * 16 + NT * 1024;      // rows whose scales are loaded, bytes of a set
+  // the sets that S steps under way and the one that is multiplied may touch
+  static constexpr int sets(int steps) { return (steps + 2) / 4 + 1; }
+  static constexpr int bytes(int steps) { return steps * STEP + sets(steps) * SCALES; }
+  static constexpr int fit(int lds) { int n = 2; while (n < 8 && bytes(n + 1) <= lds) ++n; return n; }
+};
+template <typename T, int MT, int NT, int EPI, int S>
+__global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using R = MxRing<MT, NT>;
+  constexpr int SCB = R::SCALES, SETS = R::sets(S);
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[R::bytes(S)];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int KB = a.KB, SS = (KB + 3) >> 2, ntiles = (a.N + 15) >> 4, half = ntiles >> 1;
+  int row0 = blockIdx.x * (16 * MT), end = a.M, group = 0;
+  if (a.tiles != nullptr) {
+    const int* d = a.tiles + 3 * blockIdx.x;
+    const int rows = __builtin_amdgcn_readfirstlane(d[2]);
+    if (rows <= 0) return;
+    group = min(max(__builtin_amdgcn_readfirstlane(d[0]), 0), a.groups - 1);
+    row0 = min(max(__builtin_amdgcn_readfirstlane(d[1]), 0), a.M - 1);
+    end = min(a.M, row0 + min(rows, 16 * MT));
+  }
+  // this workgroup's steps
+  const int lo = (int)((long)KB * blockIdx.z / a.ksplit), hi = (int)((long)KB * (blockIdx.z + 1) / a.ksplit);
+  int nt0[NT];                                                 // this wave's column tiles
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (EPI == MX_GLU) nt0[t] = 2 * (4 * (int)blockIdx.y + wid) + (t & 1) + (t >> 1) * half;
+    else nt0[t] = (4 * (int)blockIdx.y + wid) * NT + t;
+  }
+
+  // ---- staging.  Rows past the end, tiles past the last come as zeros from outside their descriptors
+  const unsigned wbytes = (unsigned)((long)ntiles * KB * 1024), sbytes = (unsigned)((long)ntiles * SS * 256);
+  const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.xq), 0, (int)(unsigned)((long)a.x_rows * a.ldq), 0x00020000);
+  const auto xsr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.xs), 0, (int)(unsigned)((long)a.x_rows * a.lds), 0x00020000);
+  const auto wrs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.qw + (long)group * wbytes), 0, (int)wbytes, 0x00020000);
+  const auto wsr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.ws + (long)group * sbytes), 0, (int)sbytes, 0x00020000);
+  const unsigned ldq = (unsigned)a.ldq;
+  // x: MT / 2 pieces of eight rows a wave (MT 2: one); a row's 16-byte slots XOR-ed with (row >> 1) & 7
+  constexpr int XP = MT / 2;
+  unsigned xoff[XP], soff[R::XR / 64];
+  auto row_of = [&](int m) {                                   // of x behind row m of this workgroup
+    int row = min(row0 + m, end - 1);
+    if (a.src != nullptr) row = min(max(a.src[row], 0), a.x_rows - 1);
+    return (unsigned)row;
+  };
+#pragma unroll
+  for (int i = 0; i < XP; ++i) {
+    const int m = 8 * (XP * wid + i) + (lane >> 3);
+    xoff[i] = row_of(m) * ldq + 16 * ((lane & 7) ^ ((m >> 1) & 7));
+  }
+  // scales of x: 64 lanes x 4 bytes, 16 rows of 16 bytes each; MT < 4: the last rows again
+#pragma unroll
+  for (int i = 0; i < R::XR / 64; ++i) soff[i] = row_of(min(16 * (R::XR / 64 * wid + i) + (lane >> 2), 16 * MT - 1)) * (unsigned)a.lds + 4 * (lane & 3);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (loads of src: nothing of them among the counted ones)
+  constexpr int PER = XP + NT;                                 // loads of a wave and step, without scales
+  auto stage = [&](int k, int buf) {
+    unsigned char* const to = smem + buf * R::STEP;
+#pragma unroll
+    for (int i = 0; i < XP; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mx_lds_void*)(to + (XP * wid + i) * 1024), 16, xoff[i], k * 128, 0, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (mx_lds_void*)(to + R::X + (wid * NT + t) * 1024), 16,
+                                               16u * lane + (unsigned)nt0[t] * (unsigned)(KB * 1024), k * 1024, 0, 0);
+  };
+  auto stage_scales = [&](int ss, int set) {
+    unsigned char* const to = smem + S * R::STEP + set * SCB;
+#pragma unroll
+    for (int i = 0; i < R::XR / 64; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xsr, (mx_lds_void*)(to + (R::XR / 64 * wid + i) * 256), 4, soff[i], ss * 16, 0, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mx_lds_void*)(to + R::XR * 16 + (wid * NT + t) * 256), 4,
+                                               4u * lane + (unsigned)nt0[t] * (unsigned)(SS * 256), ss * 256, 0, 0);
+  };
+
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int swz = (r >> 1) & 7, so0 = (q ^ swz) << 4, so1 = ((4 + q) ^ swz) << 4;
+  // set of four steps ss: (ss - first) mod SETS; a step's buffer: (k - lo) mod S
+  const int first = lo >> 2;
+  int sbuf = 0, sset = 0;                                      // where the next step's and the next set's loads go
+  auto issue = [&](int k) {                                    // everything of step k
+    if (k == lo || (k & 3) == 0) {
+      stage_scales(k >> 2, sset);
+      sset = sset + 1 == SETS ? 0 : sset + 1;
+    }
+    stage(k, sbuf);
+    sbuf = sbuf + 1 == S ? 0 : sbuf + 1;
+  };
+  for (int k = lo; k < min(lo + S - 1, hi); ++k) issue(k);
+  int buf = 0, set = 0;
+  for (int k = lo; k < hi; ++k) {
+    __builtin_amdgcn_sched_barrier(0);
+    // at most the S - 2 steps behind this one are in flight (scales among them make the count stricter); near the end fewer: all
+    if (k + S - 2 < hi) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * PER) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (k + S - 1 < hi) issue(k + S - 1);
+    const unsigned char* const at = smem + buf * R::STEP;
+    const unsigned char* const sc = smem + S * R::STEP + set * SCB;
+    mx_u32x4 w[NT];
+    uint32_t sw[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      w[t] = *reinterpret_cast<const mx_u32x4*>(at + R::X + (wid * NT + t) * 1024 + lane * 16);
+      sw[t] = sc[R::XR * 16 + (wid * NT + t) * 256 + lane * 4 + (k & 3)];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const unsigned char* const p = at + (16 * i + r) * 128;
+      const mx_i32x8 x = mx_fragment(p + so0, p + so1);
+      const uint32_t sx = sc[(16 * i + r) * 16 + 4 * (k & 3) + q];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t][i] = mx_mfma(w[t], x, acc[t][i], sw[t], sx);
+    }
+    buf = buf + 1 == S ? 0 : buf + 1;
+    if ((k & 3) == 3) set = set + 1 == SETS ? 0 : set + 1;
+  }
+
+  // ---- lane (r, q): columns 4 q .. + 3 of tile t, row 16 i + r
+  if constexpr (EPI == MX_GLU) {
+    const int n0 = 32 * (4 * blockIdx.y + wid), n1 = n0 + (a.N >> 1);
+    if (n0 >= a.N >> 1) return;
+    float b0[2][4], b1[2][4];
+    mx_bias<T>(b0, a.bias, (long)group * a.N, n0, a.N, q);
+    mx_bias<T>(b1, a.bias, (long)group * a.N, n1, a.N, q);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = row0 + 16 * i + r;
+      float v[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = mx_glu(acc[j][i][e] + b0[j][e], acc[2 + j][i][e] + b1[j][e], a.limit, a.alpha);
+      mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n0, a.os + (long)m * a.ldos + (n0 >> 5), v, lane, m < end);
+    }
+  } else {
+    const T* bias = a.bias == nullptr ? nullptr : (const T*)a.bias + (long)group * a.N;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = 16 * nt0[t] + 4 * q;
+      if (n >= a.N) continue;
+      f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (EPI == MX_OUT && bias != nullptr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = (float)bias[n + e];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int m = row0 + 16 * i + r;
+        if (m >= end) continue;
+        if constexpr (EPI == MX_SLAB) {
+          *reinterpret_cast<f32x4*>(a.partial + ((long)blockIdx.z * a.M + m) * a.N + n) = acc[t][i];
+        } else {
+          typename Vec4<T>::type o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = (T)(acc[t][i][e] + b[e]);
+          *reinterpret_cast<typename Vec4<T>::type*>((T*)a.out + (long)m * a.ldo + n) = o;
+        }
+      }
+    }
+  }
+#endif
+}
+
 // y = sum of the slabs + bias
 template <typename T>
 __global__ __launch_bounds__(256) void mx_reduce_kernel(T* __restrict__ out, long ldo, const float* __restrict__ partial,
@@ -645,22 +826,53 @@ int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
   return 0;
 }
 
+// row_tiles 2, 4 or 8, n_tiles 2 or 4 (MX_GLU: 4), waves 1: as many steps ahead as half of a unit's LDS holds, 2: as all of it holds
+template <typename T, int EPI, int MT, int NT, int LDS>
+int mx_ring_go(const MxArgs& a, hipStream_t st) {
+  constexpr int S = MxRing<MT, NT>::fit(LDS);
+  const int ntiles = (a.N + 15) / 16, per = 4 * NT;
+  dim3 grid(a.tiles != nullptr ? a.num_tiles : (a.M + 16 * MT - 1) / (16 * MT), (ntiles + per - 1) / per, a.ksplit);
+  if (grid.y > 65535 || grid.z > 65535) return -7;
+  mx_ring_kernel<T, MT, NT, EPI, S><<<grid, 256, 0, st>>>(a);
+  HIP_LAUNCH_CHECK();
+  return 0;
+}
+template <typename T, int EPI>
+int mx_ring(const MxArgs& a, int mt, int nt, int deep, hipStream_t st) {
+  const long lim = (1L << 32) - 64;
+  if (a.x16 != nullptr || (long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim) return -8;
+#define GO(M_, N_)                                                                     \
+  if (mt == M_ && nt == N_)                                                            \
+    return deep ? mx_ring_go<T, EPI, M_, N_, 158 * 1024>(a, st) : mx_ring_go<T, EPI, M_, N_, 79 * 1024>(a, st)
+  if constexpr (EPI != MX_GLU) {
+    GO(2, 2);
+    GO(4, 2);
+    GO(8, 2);
+  }
+  GO(2, 4);
+  GO(4, 4);
+  GO(8, 4);
+#undef GO
+  return -6;
+}
+
 template <typename T>
 int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t st) {
   if (mt == 16) {
     if (a.ksplit != 1 || a.src != nullptr || a.x16 != nullptr) return -1;
     return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : -1;
   }
-  if (epi == MX_GLU) return mx_stream<T, MX_GLU>(a, mt, nt, waves, st);
+  const bool ring = waves <= 2;
+  if (epi == MX_GLU) return ring ? mx_ring<T, MX_GLU>(a, mt, nt, waves == 2, st) : mx_stream<T, MX_GLU>(a, mt, nt, waves, st);
   if (epi == MX_SLAB || a.ksplit > 1) {
-    const int rc = mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
+    const int rc = ring ? mx_ring<T, MX_SLAB>(a, mt, nt, waves == 2, st) : mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
     if (rc != 0 || epi == MX_SLAB) return rc;
     const long n = (long)a.M * (a.N / 4);
     mx_reduce_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>((T*)a.out, a.ldo, a.partial, (const T*)a.bias, a.M, a.N, a.ksplit);
     HIP_LAUNCH_CHECK();
     return 0;
   }
-  return mx_stream<T, MX_OUT>(a, mt, nt, waves, st);
+  return ring ? mx_ring<T, MX_OUT>(a, mt, nt, waves == 2, st) : mx_stream<T, MX_OUT>(a, mt, nt, waves, st);
 }
 
 }  // namespace

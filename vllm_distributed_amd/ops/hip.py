@@ -2568,11 +2568,14 @@ def mx_plan(m: int, n: int, kb: int, big: bool, gated: bool = False) -> Tuple[in
         # 10240 22.3, 18.9, 15.4; 4 of 4096 into 28672 18.4, 15.8, 14.9; 8 of 8192 into 1280 7.6, 8.7, 10.4
         nt = 4 if gated or tiles >= (640 if m > 4 else 1536) else 2 if tiles >= (256 if m > 4 else 448) else 1
         return _mx_shape(1, nt, 4 if nt == 4 and tiles >= 1024 else 8), 1
-    mt = 2 if m <= 32 else 4
-    if gated:
-        return _mx_shape(mt, 4, 4), 1
-    wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
-    return _mx_shape(mt, 4, 4), max(1, min((512 + wgs - 1) // wgs, kb // 8))
+    if not big:
+        mt = 2 if m <= 32 else 4
+        wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
+        return _mx_shape(mt, 4, 4), 1 if gated else max(1, min((512 + wgs - 1) // wgs, kb // 8))
+    mt = 2 if m <= 32 else 4 if m <= 64 else 8
+    nt = 4 if gated else 2
+    wgs = ((n + 64 * nt - 1) // (64 * nt)) * ((m + 16 * mt - 1) // (16 * mt))
+    return _mx_shape(mt, nt, 1), 1 if gated else max(1, min((512 + wgs - 1) // wgs, kb // 8))
 
 
 def mx_fused_ok(m: int, kb: int) -> bool:
