@@ -596,7 +596,9 @@ int mx_big(const MxArgs& a, hipStream_t st) {
 // tiles, its four waves NT of them each and all of the rows; K in steps of 128, split over the grid.  x and the weights of S steps are in
 // LDS or on their way to it, straight from memory: the loads of the step that is S - 1 ahead go out while one is multiplied, so
 // (S - 1) (2 MT + 4 NT) KiB a workgroup are in flight, and the bytes of the weights are the time until the matrix cores are.
-// A step is one barrier: behind it every wave's loads of the step are there and every wave has read the step before.
+// A step is one barrier: behind it every wave's loads of the step are there and every wave has read the step before.  (Reading the next
+// step's fragments while this one's are multiplied takes a step off what is in flight, and was slower at every size: 8192 x 28672 by
+// 100 rows 43 -> 53 us.)
 // Scales come 16 bytes a row (four steps) at a time, with the first step of each four, into sets of their own.
 // MX_GLU: NT 4, a wave's tiles are two of the gate and the same two of the up half - a block of 32 columns.
 template <int MT, int NT> struct MxRing {
@@ -789,6 +791,34 @@ __global__ __launch_bounds__(256) void mx_reduce_kernel(T* __restrict__ out, lon
   *reinterpret_cast<typename Vec4<T>::type*>(out + m * ldo + n) = o;
 }
 
+// rows of gated activations in 8 bits from the slabs of [gate | up]; a thread has 8 columns, a quad a block
+template <typename T>
+__global__ __launch_bounds__(256) void mx_reduce_glu_kernel(uint8_t* __restrict__ out, long ldo, uint8_t* __restrict__ os, long ldos,
+                                                            const float* __restrict__ partial, const T* __restrict__ bias, int M, int N,
+                                                            int ksplit, float limit, float alpha) {
+  const long i = blockIdx.x * 256L + threadIdx.x;
+  const int half = N >> 1, per_row = half >> 3;
+  if (i >= (long)M * per_row) return;                          // (per_row is a multiple of 4: quads agree)
+  const int m = (int)(i / per_row), c = (int)(i - (long)m * per_row) * 8;
+  float g[8], u[8], v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    g[e] = bias ? (float)bias[c + e] : 0.f;
+    u[e] = bias ? (float)bias[half + c + e] : 0.f;
+  }
+  for (int k = 0; k < ksplit; ++k) {
+    const float* const p = partial + ((long)k * M + m) * N + c;
+    float a[8], b[8];
+    mx_load8(p, a);
+    mx_load8(p + half, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { g[e] += a[e]; u[e] += b[e]; }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = mx_glu(g[e], u[e], limit, alpha);
+  mx_store8(out + m * ldo + c, os + m * ldos + (c >> 5), v);
+}
+
 // shapes of a launch of the streaming kernel: one row tile with 1 or 2 column tiles and 8 waves (not MX_GLU) or 4 and 8, and with 4 column
 // tiles and 4 waves 1, 2 or 4 row tiles
 template <typename T, int EPI>
@@ -826,10 +856,11 @@ int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
   return 0;
 }
 
-// row_tiles 2, 4 or 8, n_tiles 2 or 4 (MX_GLU: 4), waves 1: as many steps ahead as half of a unit's LDS holds, 2: as all of it holds
-template <typename T, int EPI, int MT, int NT, int LDS>
+// row_tiles 2, 4 or 8, n_tiles 2 (MX_GLU: 4), waves 1.  As many steps as fit half of a unit's LDS: two workgroups a unit hide each other's
+// barriers (twice the steps in one workgroup's: 8192 x 28672 by 48 rows 31 -> 35 us, 6144 x 4096 by 411 25.3 -> 25.7)
+template <typename T, int EPI, int MT, int NT>
 int mx_ring_go(const MxArgs& a, hipStream_t st) {
-  constexpr int S = MxRing<MT, NT>::fit(LDS);
+  constexpr int S = MxRing<MT, NT>::fit(MT * NT <= 16 ? 80 * 1024 : 158 * 1024);
   const int ntiles = (a.N + 15) / 16, per = 4 * NT;
   dim3 grid(a.tiles != nullptr ? a.num_tiles : (a.M + 16 * MT - 1) / (16 * MT), (ntiles + per - 1) / per, a.ksplit);
   if (grid.y > 65535 || grid.z > 65535) return -7;
@@ -838,21 +869,15 @@ int mx_ring_go(const MxArgs& a, hipStream_t st) {
   return 0;
 }
 template <typename T, int EPI>
-int mx_ring(const MxArgs& a, int mt, int nt, int deep, hipStream_t st) {
+int mx_ring(const MxArgs& a, int mt, int nt, hipStream_t st) {
   const long lim = (1L << 32) - 64;
-  if (a.x16 != nullptr || (long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim) return -8;
-#define GO(M_, N_)                                                                     \
-  if (mt == M_ && nt == N_)                                                            \
-    return deep ? mx_ring_go<T, EPI, M_, N_, 158 * 1024>(a, st) : mx_ring_go<T, EPI, M_, N_, 79 * 1024>(a, st)
-  if constexpr (EPI != MX_GLU) {
-    GO(2, 2);
-    GO(4, 2);
-    GO(8, 2);
+  constexpr int NT = EPI == MX_GLU ? 4 : 2;
+  if (a.x16 != nullptr || (long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim || nt != NT) return -8;
+  switch (mt) {
+    case 2: return mx_ring_go<T, EPI, 2, NT>(a, st);
+    case 4: return mx_ring_go<T, EPI, 4, NT>(a, st);
+    case 8: return mx_ring_go<T, EPI, 8, NT>(a, st);
   }
-  GO(2, 4);
-  GO(4, 4);
-  GO(8, 4);
-#undef GO
   return -6;
 }
 
@@ -862,17 +887,26 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t
     if (a.ksplit != 1 || a.src != nullptr || a.x16 != nullptr) return -1;
     return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : -1;
   }
-  const bool ring = waves <= 2;
-  if (epi == MX_GLU) return ring ? mx_ring<T, MX_GLU>(a, mt, nt, waves == 2, st) : mx_stream<T, MX_GLU>(a, mt, nt, waves, st);
+  const bool ring = waves == 1;
+  if (epi == MX_GLU && a.ksplit > 1) {
+    const int rc = ring ? mx_ring<T, MX_SLAB>(a, mt, nt, st) : mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
+    if (rc != 0) return rc;
+    const long n = (long)a.M * (a.N / 16);
+    mx_reduce_glu_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>((uint8_t*)a.out, a.ldo, a.os, a.ldos, a.partial, (const T*)a.bias,
+                                                                        a.M, a.N, a.ksplit, a.limit, a.alpha);
+    HIP_LAUNCH_CHECK();
+    return 0;
+  }
+  if (epi == MX_GLU) return ring ? mx_ring<T, MX_GLU>(a, mt, nt, st) : mx_stream<T, MX_GLU>(a, mt, nt, waves, st);
   if (epi == MX_SLAB || a.ksplit > 1) {
-    const int rc = ring ? mx_ring<T, MX_SLAB>(a, mt, nt, waves == 2, st) : mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
+    const int rc = ring ? mx_ring<T, MX_SLAB>(a, mt, nt, st) : mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
     if (rc != 0 || epi == MX_SLAB) return rc;
     const long n = (long)a.M * (a.N / 4);
     mx_reduce_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>((T*)a.out, a.ldo, a.partial, (const T*)a.bias, a.M, a.N, a.ksplit);
     HIP_LAUNCH_CHECK();
     return 0;
   }
-  return ring ? mx_ring<T, MX_OUT>(a, mt, nt, waves == 2, st) : mx_stream<T, MX_OUT>(a, mt, nt, waves, st);
+  return ring ? mx_ring<T, MX_OUT>(a, mt, nt, st) : mx_stream<T, MX_OUT>(a, mt, nt, waves, st);
 }
 
 }  // namespace
@@ -882,10 +916,11 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t
 // Or xq null: x16, rows of K columns of the model type (ldx elements apart, a multiple of 8), K % 32 == 0, at most 128 KB, quantised
 // inside: at most 16 rows, of which a workgroup's part fits 48 KiB; no tiles.
 // epi 0: out [M][N] of the model type, rows ldo elements apart (ksplit > 1: through partial [ksplit][M][N]); 1: partial alone;
-// 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales, ksplit 1; limit 0: SiLU.
-// tiles [num_tiles][3] (matrix, first row, rows) or null; src [M] or null: the row of x behind each row.  shape: 16-row tiles a
-// workgroup takes (1, 2 or 4; of `tiles` at most 16 times as many rows each) + 256 times its 16-column tiles + 65536 times its waves;
-// 16: the kernel of 256-row tiles (ksplit 1, src null, x_rows ldq and a matrix's bytes below 2^32, lds a multiple of 16).
+// 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales (ksplit > 1: through partial); limit 0: SiLU.
+// tiles [num_tiles][3] (matrix, first row, rows; ksplit 1) or null; src [M] or null: the row of x behind each row.
+// shape: 16-row tiles a workgroup takes (of `tiles` at most 16 times as many rows each) + 256 times its 16-column tiles + 65536 times its
+// waves for the streaming kernel (mx_stream);  row tiles 2, 4 or 8 + 256 times 2 (4 where epi is 2 and ksplit 1) + 65536: the ring of LDS;
+// 16: the kernel of 256-row tiles (ksplit 1, src null).  The last two: x_rows ldq and a matrix's bytes below 2^32, lds a multiple of 16.
 VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* partial, const void* xq, long ldq, const void* xs, long lds,
                             int x_rows, const void* x16, long ldx, int K, const void* qw, const void* ws, const void* bias, int M, int N,
                             int KB, int ksplit, int epi, float limit, float alpha, const int* tiles, int num_tiles, int groups,
@@ -898,7 +933,7 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
   } else if (x_rows <= 0 || (src == nullptr && x_rows < M) || ldq % 128 || ldq < 128L * KB || lds < 4L * KB || (uintptr_t)xq % 16) {
     return -1;
   }
-  if (epi == MX_GLU && (N % 256 || ksplit != 1 || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
+  if (epi == MX_GLU && (N % 256 || (ksplit > 1 && partial == nullptr) || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
   if (epi == MX_OUT && (ldo % 8 || ldo < N || (uintptr_t)out % 16 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;
   if ((ksplit > 1 || epi == MX_SLAB) && tiles != nullptr) return -1;

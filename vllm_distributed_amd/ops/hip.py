@@ -2557,25 +2557,52 @@ def _mx_shape(mt: int, nt: int, waves: int) -> int:
     return mt + 256 * nt + 65536 * waves
 
 
+# us of a step of the ring kernel's workgroups by (16-row tiles, column tiles of a wave): of one alone on a unit, of each that shares one;
+# fitted with the other constants of _mx_estimate to 16 shapes of 1000 to 57344 columns and 1024 to 28672 of reduction by 8 to 2048 rows
+# (the choice is within 2 % of the best of them on average, 28 % at worst)
+_MX_RING = {(2, 2): (0.30, 0.31), (4, 2): (0.49, 0.29), (8, 2): (0.96, 0.77), (2, 4): (0.39, 0.41), (4, 4): (0.55, 0.46)}
+
+
+def _mx_estimate(m: int, n: int, kb: int, mt: int, nt: int, ksplit: int) -> float:
+    """Expected us of a product; ``mt`` ``MX_BIG``: 256-row tiles, whose steps slow down as they fill the chip."""
+    if mt == MX_BIG:
+        tiles = -(-m // 256) * -(-n // 256)
+        return -(-tiles // 256) * (kb * (1.02 + 0.3 * min(1.0, max(0.0, (tiles - 128) / 128))) + 6)
+    load = -(-n // (64 * nt)) * -(-m // (16 * mt)) * ksplit / 256
+    alone, shared = _MX_RING[mt, nt]
+    t = 3.5 + -(-kb // ksplit) * max(alone, shared * (math.ceil(load) if load <= 2 else load + 0.5))
+    t = max(t, n * kb * 128 * 17 / 32 / 4.9e6 + 3)
+    return t if ksplit == 1 else t + 2.2 + ksplit * m * n * 8 / 5.5e6
+
+
+@functools.lru_cache(maxsize=4096)
 def mx_plan(m: int, n: int, kb: int, big: bool, gated: bool = False) -> Tuple[int, int]:
-    """(shape of the launch, K split) of ``m`` rows against ``n`` columns; ``big``: the kernel of 256-row tiles may be chosen."""
-    if big and m > 512:
-        return MX_BIG, 1
+    """(shape of the launch, K split) of ``m`` rows against ``n`` columns; ``big``: operands are within 32-bit offsets, as every kernel
+    but the streaming one wants them."""
     tiles = (n + 15) // 16
-    if m <= 16:
-        # Column tiles a workgroup takes: more read x less often, fewer spread over the chip.  us with 1, 2 and 4: one row of 4096 into
-        # 6144 columns 5.5, 5.6, 6.6; of 28672 into 8192 20.7, 20.2, 23.9; 13 rows of 8192 into 8192 15.4, 11.2, 13.7; 16 of 8192 into
-        # 10240 22.3, 18.9, 15.4; 4 of 4096 into 28672 18.4, 15.8, 14.9; 8 of 8192 into 1280 7.6, 8.7, 10.4
-        nt = 4 if gated or tiles >= (640 if m > 4 else 1536) else 2 if tiles >= (256 if m > 4 else 448) else 1
+    if not big or (m <= 16 and not (m > 8 and (kb >= 112 or n * kb >= 850000))):
+        if m > 16:
+            mt = 2 if m <= 32 else 4
+            wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
+            return _mx_shape(mt, 4, 4), max(1, min((512 + wgs - 1) // wgs, kb // 8))
+        # Column tiles a workgroup takes: more read x less often, fewer spread over the chip.  us with 1, 2 and 4: 16 rows of 8192 into 1280
+        # columns 10.8, 11.6, 14.0; of 4096 into 6144 9.3, 8.0, 9.6; of 8192 into 8192 15.4, 12.5, 15.1; 8 of 4096 into 28672 18.8, 15.8, 15.2;
+        # one of 8192 into 57344 38.9, 36.7, 44.4.  More than 8 rows of long reductions or large weights go to the ring: 16 of 28672 into
+        # 8192 33 and 27, of 8192 into 57344 50 and 46, of 8192 into 8192 12.5 and 14.1
+        nt = 4 if gated or (tiles > 1024 and m > 2) else 2 if tiles > 256 else 1
         return _mx_shape(1, nt, 4 if nt == 4 and tiles >= 1024 else 8), 1
-    if not big:
-        mt = 2 if m <= 32 else 4
-        wgs = ((n + 63) // 64) * ((m + 16 * mt - 1) // (16 * mt))
-        return _mx_shape(mt, 4, 4), 1 if gated else max(1, min((512 + wgs - 1) // wgs, kb // 8))
-    mt = 2 if m <= 32 else 4 if m <= 64 else 8
-    nt = 4 if gated else 2
-    wgs = ((n + 64 * nt - 1) // (64 * nt)) * ((m + 16 * mt - 1) // (16 * mt))
-    return _mx_shape(mt, nt, 1), 1 if gated else max(1, min((512 + wgs - 1) // wgs, kb // 8))
+    best, plan = _mx_estimate(m, n, kb, MX_BIG, 0, 1), (MX_BIG, 1)
+    for mt in (2, 4, 8):
+        if 16 * mt > max(32, 2 * m):
+            break
+        for ksplit in (1, 2, 4, 8, 16):
+            nt = 4 if gated and ksplit == 1 else 2
+            if (mt, nt) not in _MX_RING or (ksplit > 1 and kb // ksplit < 3):
+                continue
+            t = _mx_estimate(m, n, kb, mt, nt, ksplit)
+            if t < best:
+                best, plan = t, (_mx_shape(mt, nt, 1), ksplit)
+    return plan
 
 
 def mx_fused_ok(m: int, kb: int) -> bool:
@@ -2642,15 +2669,16 @@ def mx_gate_up(x, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float,
     _, nt, kb = _mx_check(x, w, bias, False)
     r = _mx_gated_out(x, w, m)
     if m:
-        _mx_gemm(2, x, w, 1, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None,
-                 mx_plan(m, w.rows, kb, mx_big_ok(m, nt, kb), True), limit, alpha)
+        plan = mx_plan(m, w.rows, kb, mx_big_ok(m, nt, kb), True)
+        partial = torch.empty((plan[1], m, w.rows), dtype=torch.float32, device=x.device) if plan[1] > 1 else None
+        _mx_gemm(2, x, w, 1, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], partial, plan, limit, alpha)
     return r
 
 
 def mx_tile_rows(slots: int, experts: int) -> int:
     """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices."""
     avg = slots / max(1, experts)
-    return 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 96 else 256
+    return 16 if avg <= 12 else 32 if avg <= 32 else 64 if avg <= 96 else 256
 
 
 def mx_sorted_ok(slots: int, w: quant.MxWeight) -> bool:
