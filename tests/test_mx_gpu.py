@@ -312,7 +312,7 @@ def make_experts(e, n, k, halves=1):
 
 
 @pytest.mark.parametrize("t,e,k,h,inter,limit", [(1, 8, 2, 128, 128, 0.0), (16, 128, 4, 288, 160, 7.0), (9, 4, 4, 160, 128, 7.0),
-                                                 (70, 8, 2, 256, 384, 0.0), (300, 5, 3, 96, 96, 7.0), (1200, 4, 2, 256, 128, 0.0), (513, 3, 2, 160, 416, 7.0)])
+                                                 (70, 8, 2, 256, 384, 0.0), (40, 4, 2, 416, 160, 7.0), (150, 4, 2, 160, 288, 7.0), (300, 5, 3, 96, 96, 7.0), (1200, 4, 2, 256, 128, 0.0), (513, 3, 2, 160, 416, 7.0)])
 def test_experts(t, e, k, h, inter, limit):
     from vllm_distributed_amd import ops
     from vllm_distributed_amd.ops import quant

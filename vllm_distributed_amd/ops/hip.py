@@ -2676,9 +2676,12 @@ def mx_gate_up(x, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float,
 
 
 def mx_tile_rows(slots: int, experts: int) -> int:
-    """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices."""
+    """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices: 16 stream their weights, 32 and 64 share them through
+    the ring, 256 are the large tiles.  us of gate and up and down in tiles of 16, 32, 64 and 256: 128 experts of 2880 x 2880 with 8 rows
+    each 293, 320, 338, -, with 16 456, 337, 349, -, with 32 798, 426, 367, 757; 32 experts with 64 363, 179, 154, 218, with 128 668, 318,
+    223, 230, with 250 -, 627, 419, 335; 8 of 4096 x 14336 with 128 -, 543, 362, 350."""
     avg = slots / max(1, experts)
-    return 16 if avg <= 12 else 32 if avg <= 32 else 64 if avg <= 96 else 256
+    return 16 if avg <= 10 else 32 if avg <= 24 else 64 if avg <= 128 else 256
 
 
 def mx_sorted_ok(slots: int, w: quant.MxWeight) -> bool:
@@ -2692,21 +2695,25 @@ def mx_sorted_rows(x, src_row: torch.Tensor) -> quant.MxRows:
     return x.take(src_row) if isinstance(x, quant.MxRows) else mx_quantize(x, 8, src_row=src_row)
 
 
-def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], device: torch.device) -> int:
+def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], rows: quant.MxRows, nt: int, kb: int, gated: bool) -> int:
     assert tiles.dtype == torch.int32 and tiles.dim() == 2 and tiles.shape[1] == 3 and tiles.is_contiguous()
     assert src is None or (src.dtype == torch.int32 and src.dim() == 1 and src.is_contiguous())
     assert tile_rows in (16, 32, 64, 256), tile_rows
     assert tile_rows < 256 or src is None, "tiles of 256 rows: the rows themselves, in order"
-    _mx_device(device.index, tiles, src)
-    return MX_BIG if tile_rows == 256 else _mx_shape(tile_rows // 16, 4, 4)
+    _mx_device(rows.payload.get_device(), tiles, src)
+    if tile_rows == 256:
+        return MX_BIG
+    if tile_rows > 16 and mx_big_ok(rows.payload.shape[0], nt, kb):
+        return _mx_shape(tile_rows // 16, 4 if gated else 2, 1)
+    return _mx_shape(tile_rows // 16, 4, 4)
 
 
 def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor] = None,
                       src_row: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Product of rows sorted by matrix (``moe_align``) with ``w``'s matrices; ``src_row``: the rows are ``rows[src_row]``.  Rows of no
     tile stay unwritten."""
-    mt = _mx_tiles(tiles, tile_rows, src_row, rows.device)
-    groups, _, kb = _mx_check(rows, w, bias, True)
+    groups, nt, kb = _mx_check(rows, w, bias, True)
+    mt = _mx_tiles(tiles, tile_rows, src_row, rows, nt, kb, False)
     out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=rows.dtype, device=rows.device)
     if out.shape[0]:
         _mx_gemm(0, rows, w, groups, kb, bias, out, w.rows, None, 0, None, (mt, 1), tiles=tiles, src=src_row)
@@ -2715,8 +2722,8 @@ def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor
 
 def mx_grouped_gate_up(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor],
                        limit: float, alpha: float, src_row: Optional[torch.Tensor] = None) -> quant.MxRows:
-    mt = _mx_tiles(tiles, tile_rows, src_row, rows.device)
-    groups, _, kb = _mx_check(rows, w, bias, True)
+    groups, nt, kb = _mx_check(rows, w, bias, True)
+    mt = _mx_tiles(tiles, tile_rows, src_row, rows, nt, kb, True)
     r = _mx_gated_out(rows, w, rows.shape[0] if src_row is None else src_row.numel())
     if r.shape[0]:
         _mx_gemm(2, rows, w, groups, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], None, (mt, 1), limit, alpha, tiles,
