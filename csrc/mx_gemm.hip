@@ -23,7 +23,7 @@ struct MxArgs {
   const uint8_t* ws;
   void* out; long ldo;              // MX_OUT: rows of y; MX_GLU: rows of 8-bit elements
   uint8_t* os; long ldos;           // MX_GLU: their scales
-  float* partial;                   // MX_SLAB: [ksplit][M][N]
+  float* partial;                   // MX_SLAB: 32-bit rows [ksplit][M][N]
   const void* bias;                 // [N] of the model type (MX_GLU: [gate ; up]), or null
   int M, N, KB, ksplit;             // KB: steps of 128 columns
   float limit, alpha;               // MX_GLU: limit 0: SiLU
@@ -244,13 +244,16 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(const MxArgs a) {
       const int t = j % NT, i = j / NT;
       const int n = 16 * (NT * (int)blockIdx.x + t) + 4 * q, m = 16 * i + r;
       if (n >= a.N || m >= rows) continue;
-      const f32x4 v = sum(t, i);
+      f32x4 v = sum(t, i);
+      if (bias != nullptr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += (float)bias[n + e];
       if constexpr (EPI == MX_SLAB) {
         *reinterpret_cast<f32x4*>(a.partial + ((long)blockIdx.y * a.M + row0 + m) * a.N + n) = v;
       } else {
         typename Vec4<T>::type o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (T)(v[e] + (bias ? (float)bias[n + e] : 0.f));
+        for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
         *reinterpret_cast<typename Vec4<T>::type*>((T*)a.out + (row0 + m) * a.ldo + n) = o;
       }
     }
@@ -301,7 +304,7 @@ __device__ __forceinline__ void mx_bias(float (&b)[2][4], const void* bias, long
 //  * A wave has 128 x 64 outputs as four quadrants of 64 x 32, quadrant (mq, nq) from images A<mq> and B<nq>; a step is four phases of
 //    eight matrix instructions, one quadrant each, every fragment read once.  Even steps go A0 B0, A1 B0, A1 B1, A0 B1, odd ones begin
 //    with A1: registers of the half that a step begins with are free a phase before it, so the 20 fragment reads of a step spread as
-//    6, 6, 4, 4 over its phases and stay below the matrix instructions' time in each (as 8, 8, 2, 2: 2780 TFLOP/s instead of ____).
+//    6, 6, 4, 4 over its phases and stay below the matrix instructions' time in each (as 8, 8, 2, 2: 2780 TFLOP/s instead of 2880).
 //  * The loads are one stream that never drains.  Of step t are issued: B0 in phase 1 of step t - 2, the first A half in 2, the second in
 //    3, B1 in phase 0 of step t - 1; each at least two phases after the image before it was read.  A phase waits for what the next one
 //    reads, all but the newest six loads of a wave (an A image is two, a B image one).  It runs on through the output tiles.
@@ -533,6 +536,17 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[j][e] = mx_glu(a0[i][j][e] + b0[j][e], a1[i][j][e] + b1[j][e], a.limit, a.alpha);
           mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n0, a.os + (long)m * a.ldos + (n0 >> 5), v, eln, m < cend);
+        } else if constexpr (EPI == MX_SLAB) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              f32x4 v = h ? a1[i][j] : a0[i][j];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] += h ? b1[j][e] : b0[j][e];
+              const int n = (h ? n1 : n0) + 16 * j + 4 * eq;
+              if (m < cend && n < a.N) *reinterpret_cast<f32x4*>(a.partial + (long)m * a.N + n) = v;
+            }
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -587,7 +601,8 @@ int mx_big(const MxArgs& a, hipStream_t st) {
   const int cus = mx_num_cus() / 8;
   const unsigned grid = 8 * (unsigned)(per < cus ? per : cus);
   if (a.tiles != nullptr) mx_big_kernel<T, EPI, true><<<grid, 512, 0, st>>>(a, ntm, ntn);
-  else mx_big_kernel<T, EPI, false><<<grid, 512, 0, st>>>(a, ntm, ntn);
+  else if constexpr (EPI != MX_SLAB) mx_big_kernel<T, EPI, false><<<grid, 512, 0, st>>>(a, ntm, ntn);
+  else return -6;
   HIP_LAUNCH_CHECK();
   return 0;
 }
@@ -754,7 +769,7 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
       const int n = 16 * nt0[t] + 4 * q;
       if (n >= a.N) continue;
       f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (EPI == MX_OUT && bias != nullptr)
+      if (bias != nullptr)
 #pragma unroll
         for (int e = 0; e < 4; ++e) b[e] = (float)bias[n + e];
 #pragma unroll
@@ -762,7 +777,7 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
         const int m = row0 + 16 * i + r;
         if (m >= end) continue;
         if constexpr (EPI == MX_SLAB) {
-          *reinterpret_cast<f32x4*>(a.partial + ((long)blockIdx.z * a.M + m) * a.N + n) = acc[t][i];
+          *reinterpret_cast<f32x4*>(a.partial + ((long)blockIdx.z * a.M + m) * a.N + n) = acc[t][i] + b;
         } else {
           typename Vec4<T>::type o;
 #pragma unroll
@@ -819,8 +834,34 @@ __global__ __launch_bounds__(256) void mx_reduce_glu_kernel(uint8_t* __restrict_
   mx_store8(out + m * ldo + c, os + m * ldos + (c >> 5), v);
 }
 
-// shapes of a launch of the streaming kernel: one row tile with 1 or 2 column tiles and 8 waves (not MX_GLU) or 4 and 8, and with 4 column
-// tiles and 4 waves 1, 2 or 4 row tiles
+// out[t] = sum over j of w[t][j] y[at[t k + j]], the 32-bit rows of one token's experts in order, rounded once (the rows in 16 bits would
+// add their own rounding to it: 2.4e-3 of a bf16 sum instead of 1.7e-3); slots of experts held elsewhere add nothing
+template <typename T>
+__global__ __launch_bounds__(256) void mx_combine_kernel(T* __restrict__ out, const float* __restrict__ y, const float* __restrict__ topw,
+                                                         const int* __restrict__ topi, const int* __restrict__ at, int tokens, int k,
+                                                         int H, int rows, int first, int local) {
+  const int quads = H >> 2;
+  const long i = blockIdx.x * 256L + threadIdx.x;
+  if (i >= (long)tokens * quads) return;
+  const int t = (int)(i / quads), c = (int)(i - (long)t * quads) * 4;
+  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < k; ++j) {
+    const int e = topi[t * k + j];
+    if (local >= 0 && (e < first || e >= first + local)) continue;
+    const int row = min(max(at[t * k + j], 0), rows - 1);
+    const float w = topw[t * k + j];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(y + (long)row * H + c);
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) s[e4] += w * v[e4];
+  }
+  typename Vec4<T>::type o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (T)s[e];
+  *reinterpret_cast<typename Vec4<T>::type*>(out + (long)t * H + c) = o;
+}
+
+// shapes of a launch of the streaming kernel: one row tile with 1 or 2 column tiles and 8 waves (MX_OUT) or 4 and 8 (not MX_SLAB), and with
+// 4 column tiles and 4 waves 1, 2 or 4 row tiles
 template <typename T, int EPI>
 int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
   const int ntiles = (a.N + 15) / 16;
@@ -833,16 +874,25 @@ int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
     lds = (size_t)a.M * (132 * ((a.KB + a.ksplit - 1) / a.ksplit) + 16);
     if (mt != 1 || a.M > 16 || lds > 49152 || a.tiles != nullptr) return -6;
   }
+  if constexpr (EPI == MX_SLAB)
+    if (quant || waves != 4) return -6;
   if (nt == 4 && waves == 4) {
-    if (quant) GO(1, 4, 4, true, 3);
-    else if (mt == 1) GO(1, 4, 4, false, 3);
+    if constexpr (EPI != MX_SLAB)
+      if (quant) {
+        GO(1, 4, 4, true, 3);
+        HIP_LAUNCH_CHECK();
+        return 0;
+      }
+    if (mt == 1) GO(1, 4, 4, false, 3);
     else if (mt == 2) GO(2, 4, 4, false, 2);
     else if (mt == 4) GO(4, 4, 4, false, 2);
     else return -6;
   } else if (nt == 4 && waves == 8 && mt == 1) {
-    if (quant) GO(1, 4, 8, true, 3);
-    else GO(1, 4, 8, false, 3);
-  } else if constexpr (EPI != MX_GLU) {
+    if constexpr (EPI != MX_SLAB) {
+      if (quant) GO(1, 4, 8, true, 3);
+      else GO(1, 4, 8, false, 3);
+    }
+  } else if constexpr (EPI == MX_OUT) {
     if (mt != 1 || waves != 8 || (nt != 1 && nt != 2)) return -6;
     if (nt == 1 && quant) GO(1, 1, 8, true, 6);
     else if (nt == 1) GO(1, 1, 8, false, 6);
@@ -885,11 +935,13 @@ template <typename T>
 int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t st) {
   if (mt == 16) {
     if (a.ksplit != 1 || a.src != nullptr || a.x16 != nullptr) return -1;
-    return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : -1;
+    return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : mx_big<T, MX_SLAB>(a, st);
   }
   const bool ring = waves == 1;
+  MxArgs slabs = a;                                            // (a bias goes in once, where slabs are summed)
+  if (a.ksplit > 1) slabs.bias = nullptr;
   if (epi == MX_GLU && a.ksplit > 1) {
-    const int rc = ring ? mx_ring<T, MX_SLAB>(a, mt, nt, st) : mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
+    const int rc = ring ? mx_ring<T, MX_SLAB>(slabs, mt, nt, st) : mx_stream<T, MX_SLAB>(slabs, mt, nt, waves, st);
     if (rc != 0) return rc;
     const long n = (long)a.M * (a.N / 16);
     mx_reduce_glu_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>((uint8_t*)a.out, a.ldo, a.os, a.ldos, a.partial, (const T*)a.bias,
@@ -899,7 +951,7 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t
   }
   if (epi == MX_GLU) return ring ? mx_ring<T, MX_GLU>(a, mt, nt, st) : mx_stream<T, MX_GLU>(a, mt, nt, waves, st);
   if (epi == MX_SLAB || a.ksplit > 1) {
-    const int rc = ring ? mx_ring<T, MX_SLAB>(a, mt, nt, st) : mx_stream<T, MX_SLAB>(a, mt, nt, waves, st);
+    const int rc = ring ? mx_ring<T, MX_SLAB>(slabs, mt, nt, st) : mx_stream<T, MX_SLAB>(slabs, mt, nt, waves, st);
     if (rc != 0 || epi == MX_SLAB) return rc;
     const long n = (long)a.M * (a.N / 4);
     mx_reduce_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>((T*)a.out, a.ldo, a.partial, (const T*)a.bias, a.M, a.N, a.ksplit);
@@ -915,7 +967,8 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t
 // above for `groups` matrices of N rows (padded to 16), N % 8 == 0.
 // Or xq null: x16, rows of K columns of the model type (ldx elements apart, a multiple of 8), K % 32 == 0, at most 128 KB, quantised
 // inside: at most 16 rows, of which a workgroup's part fits 48 KiB; no tiles.
-// epi 0: out [M][N] of the model type, rows ldo elements apart (ksplit > 1: through partial [ksplit][M][N]); 1: partial alone;
+// epi 0: out [M][N] of the model type, rows ldo elements apart (ksplit > 1: through partial [ksplit][M][N]); 1: partial alone (a bias with
+// ksplit 1 only);
 // 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales (ksplit > 1: through partial); limit 0: SiLU.
 // tiles [num_tiles][3] (matrix, first row, rows; ksplit 1) or null; src [M] or null: the row of x behind each row.
 // shape: 16-row tiles a workgroup takes (of `tiles` at most 16 times as many rows each) + 256 times its 16-column tiles + 65536 times its
@@ -936,7 +989,7 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
   if (epi == MX_GLU && (N % 256 || (ksplit > 1 && partial == nullptr) || ldo % 16 || (uintptr_t)out % 16 || ldo < N / 2 || os == nullptr || ldos < N / 64)) return -1;
   if (epi == MX_OUT && (ldo % 8 || ldo < N || (uintptr_t)out % 16 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;
-  if ((ksplit > 1 || epi == MX_SLAB) && tiles != nullptr) return -1;
+  if (ksplit > 1 && (tiles != nullptr || (epi == MX_SLAB && bias != nullptr))) return -1;
   if (epi < 0 || epi > 2) return -1;
   const MxArgs a = {(const uint8_t*)xq, ldq, (const uint8_t*)xs, lds, (const uint8_t*)qw, (const uint8_t*)ws, out, ldo, (uint8_t*)os, ldos,
                     partial, bias, M, N, KB, ksplit, limit, alpha, tiles, num_tiles, groups, src, x_rows, x16, ldx, K};
@@ -944,4 +997,22 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
   if (dtype == DT_BF16) return mx_dispatch<bf16_t>(a, epi, shape & 255, shape >> 8 & 255, shape >> 16, st);
   if (dtype == DT_F16) return mx_dispatch<f16_t>(a, epi, shape & 255, shape >> 8 & 255, shape >> 16, st);
   return -2;
+}
+
+// y [tokens k][H] 32-bit rows (H % 4 == 0), topw and topi [tokens][k], at [tokens k]: the row of each slot -> out [tokens][H].  local >= 0:
+// only slots of experts first .. first + local - 1
+VDAMD_API int vdamd_mx_combine(void* out, const float* y, const float* topw, const int* topi, const int* at, int tokens, int k, int H,
+                               int first, int local, int dtype, void* stream) {
+  if (tokens <= 0) return 0;
+  if (k <= 0 || H <= 0 || H % 4 || (long)tokens * k >= (1L << 31) || (uintptr_t)y % 16 || (uintptr_t)out % 8) return -1;
+  const unsigned blocks = (unsigned)(((long)tokens * (H / 4) + 255) / 256);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_BF16)
+    mx_combine_kernel<bf16_t><<<blocks, 256, 0, st>>>((bf16_t*)out, y, topw, topi, at, tokens, k, H, tokens * k, first, local);
+  else if (dtype == DT_F16)
+    mx_combine_kernel<f16_t><<<blocks, 256, 0, st>>>((f16_t*)out, y, topw, topi, at, tokens, k, H, tokens * k, first, local);
+  else
+    return -2;
+  HIP_LAUNCH_CHECK();
+  return 0;
 }

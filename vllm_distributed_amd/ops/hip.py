@@ -98,6 +98,7 @@ def load() -> ctypes.CDLL:
         "vdamd_embed_scaled": [P, P, P, F, I, I, I, I, P],
         "vdamd_mx_quantize": [P, L, P, L, P, L, L, I, I, I, P, I, I, P],
         "vdamd_mx_dequantize": [P, P, L, P, L, L, I, I, I, P],
+        "vdamd_mx_combine": [P, P, P, P, P, I, I, I, I, I, I, P],
         "vdamd_mx_rms_norm": [P, L, P, L, P, P, L, P, I, P, P, F, I, I, I, I, P],
         "vdamd_mx_gemm": [P, L, P, L, P, P, L, P, L, I, P, L, I, P, P, P, I, I, I, I, I, F, F, P, I, I, P, I, I, P],
         "vdamd_layer_norm_to": [P, P, L, P, L, P, P, F, I, I, I, I, I, P],
@@ -2709,14 +2710,31 @@ def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], 
 
 
 def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor] = None,
-                      src_row: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      src_row: Optional[torch.Tensor] = None, wide: bool = False) -> torch.Tensor:
     """Product of rows sorted by matrix (``moe_align``) with ``w``'s matrices; ``src_row``: the rows are ``rows[src_row]``.  Rows of no
-    tile stay unwritten."""
+    tile stay unwritten.  ``wide``: as the 32-bit sums."""
     groups, nt, kb = _mx_check(rows, w, bias, True)
     mt = _mx_tiles(tiles, tile_rows, src_row, rows, nt, kb, False)
-    out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=rows.dtype, device=rows.device)
+    out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=torch.float32 if wide else rows.dtype,
+                      device=rows.device)
     if out.shape[0]:
-        _mx_gemm(0, rows, w, groups, kb, bias, out, w.rows, None, 0, None, (mt, 1), tiles=tiles, src=src_row)
+        _mx_gemm(int(wide), rows, w, groups, kb, bias, None if wide else out, w.rows, None, 0, out if wide else None, (mt, 1), tiles=tiles,
+                 src=src_row)
+    return out
+
+
+def mx_combine(y: torch.Tensor, topw: torch.Tensor, topi: torch.Tensor, inv: torch.Tensor, dtype: torch.dtype, expert_start: int = 0,
+               local_experts: int = -1) -> torch.Tensor:
+    """``moe_combine`` of 32-bit rows: rounded once."""
+    t, k = topi.shape
+    h = y.shape[1]
+    assert y.dtype == torch.float32 and y.is_contiguous() and h % 4 == 0 and y.shape[0] == t * k and inv.numel() == t * k
+    assert topw.dtype == torch.float32 and topw.is_contiguous() and topw.shape == topi.shape
+    assert topi.dtype == torch.int32 and topi.is_contiguous() and inv.dtype == torch.int32 and inv.is_contiguous()
+    _mx_device(y.get_device(), topw, topi, inv)
+    out = torch.empty((t, h), dtype=dtype, device=y.device)
+    _check(_LIB.vdamd_mx_combine(out.data_ptr(), y.data_ptr(), topw.data_ptr(), topi.data_ptr(), inv.data_ptr(), t, k, h, expert_start,
+                                 local_experts, _DT[dtype], _stream()), "mx_combine")
     return out
 
 

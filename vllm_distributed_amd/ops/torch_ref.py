@@ -1202,5 +1202,5 @@ def mx_experts(rows, topw, topi, weight13, weight2, bias13, bias2, expert_start:
         h = h if bias13 is None else h + bias13[e].float()
         a = quant.mx_quantize(quant.mx_gated(h, limit, alpha), 8, rows.dtype)
         y = quant.mx_product(a, w2, None if bias2 is None else bias2[e])
-        out.index_add_(0, t, y.to(rows.dtype).float() * topw[t, j].float().unsqueeze(1))
+        out.index_add_(0, t, y * topw[t, j].float().unsqueeze(1))
     return out.to(rows.dtype)
