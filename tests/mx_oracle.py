@@ -17,7 +17,7 @@ def nearest_code(a, table):
 def blocks(x, bits):
     """x [M, K] on any device -> (codes [M, K] with the sign in the top bit, scale bytes [M, K/32], values [M, K]), on the CPU in 64 bits.
     The scale is found by trying every power of two."""
-    b = x.detach().cpu().double().reshape(x.shape[0], -1, 32)
+    b = x.detach().cpu().double().reshape(x.shape[0], x.shape[1] // 32, 32)
     table = TABLE[bits]
     finite = torch.isfinite(b).all(-1)
     a = torch.where(finite, b.abs().amax(-1), torch.zeros(b.shape[:2], dtype=torch.float64))
@@ -33,7 +33,7 @@ def blocks(x, bits):
 
 
 def pack4(code):
-    c = code.reshape(*code.shape[:-1], -1, 2).to(torch.uint8)
+    c = code.reshape(*code.shape[:-1], code.shape[-1] // 2, 2).to(torch.uint8)
     return c[..., 0] | (c[..., 1] << 4)
 
 

@@ -292,6 +292,8 @@ class ModelConfig:
     # None | awq (4-bit weights stay packed, W4A16 kernels) | awq-dequant (dense at load)
     # | fp8 (W8A8: weights quantised per channel at load, activations per token at run time)
     # | nvfp4 (E2M1 weights with e4m3 scales per 16 columns stay packed; activations stay 16-bit)
+    # | mxfp4 (microscaled: E2M1 weights with a power of two per 32 columns, quantised at load, or gpt-oss' experts as their
+    #   checkpoint holds them; activations in 8 bits with a power of two per 32 neighbours)
     quantization: Optional[str] = None
     trust_remote_code: bool = False
     revision: Optional[str] = None

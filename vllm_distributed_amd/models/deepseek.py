@@ -323,6 +323,8 @@ class DeepseekV2ForCausalLM(Qwen3MoeForCausalLM):
         if vllm_config.model_config.quantization in ("awq", "nvfp4"):
             raise NotImplementedError("4-bit DeepSeek checkpoints (the rope rows of packed projections cannot be "
                                       "re-ordered at load)")
+        if vllm_config.model_config.quantization == "mxfp4":
+            raise NotImplementedError("mxfp4 for DeepSeek: the latent attention reads its projections as 16-bit matrices")
         super().__init__(vllm_config)
         interleaved = cfg.get("model_type") == "deepseek_v2" or bool(cfg.get("rope_interleave", True))
         self.mla_perm = rope_row_permutation(cfg["qk_rope_head_dim"], cfg["qk_rope_head_dim"], interleaved)

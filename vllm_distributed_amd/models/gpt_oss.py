@@ -8,7 +8,9 @@ Checkpoints hold the experts stacked: ``gate_up_proj [E, H, 2I]`` with gate and 
 ``down_proj [E, I, H]``, and one bias row per expert for each; the original release stores the two matrices as
 MXFP4 (``*_blocks`` 16 bytes = 32 E2M1 values, ``*_scales`` one power-of-two exponent per block), which is
 widened to the model dtype at load (parity unpinned: no such checkpoint is at hand, the decoder is tested
-against an encoder written from the format's definition).
+against an encoder written from the format's definition).  With ``--quantization mxfp4`` the experts stay in 4 bits - the blocks
+as the checkpoint holds them, or quantised at load from 16-bit matrices - and multiply 8-bit microscaled rows
+(``ops.mx_experts``); the attention's projections stay in 16 bits, as they are in the checkpoint.
 
 The real shapes (hidden = intermediate = 2880) are not multiples of the 128-deep K tiles of the grouped expert
 GEMMs, so the expert matrices are zero-padded along their reduction dimension (2880 -> 2944) when they are
@@ -24,12 +26,15 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..config import VllmConfig
+from ..logger import init_logger
+from ..ops import quant
 from ..parallel.state import tensor_model_parallel_all_reduce
-from .layers.linear import ReplicatedLinear
+from .layers.linear import ReplicatedLinear, active_quant, mx_weight, quantized_linears
 from .layers.moe import FusedMoE
 from .llama import LlamaAttention, LlamaDecoderLayer, LlamaForCausalLM
 from .utils import materialize
 
+logger = init_logger(__name__)
 _EP = False
 FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -83,6 +88,14 @@ class GptOssMoE(FusedMoE):
         self.w2 = zeros(E, H, self.i_pad)
         self.b13 = zeros(E, 2 * self.i_pad)
         self.b2 = zeros(E, H)
+        spec = active_quant()
+        self.microscaled = spec is not None and spec.method == "mxfp4"
+        if self.microscaled and (H % 32 or I % 32 or E > 512 or self.top_k > 16):
+            logger.warning("experts of %d x %d on each rank do not divide into blocks of 32: they are kept in %s", H, I, dtype)
+            self.microscaled = False
+        if self.microscaled:
+            del self.w13, self.w2           # in their place the matrices as blocks, [expert][kind], until they are packed
+            self._blocks: Dict[str, List[Optional[quant.MxWeight]]] = {"gate_up_proj": [None] * E, "down_proj": [None] * E}
 
     # ------------------------------------------------------------------ loading (stacked checkpoint tensors)
     def _rows(self) -> slice:
@@ -100,7 +113,9 @@ class GptOssMoE(FusedMoE):
             e = self._local_index(eid)
             if e is None:
                 continue
-            if kind == "gate_up_proj":
+            if self.microscaled and kind in self._blocks:
+                self._blocks[kind][e] = self._pack(kind, t[eid], None if s is None else s[eid], rows)
+            elif kind == "gate_up_proj":
                 m = mxfp4_dequantize(t[eid], s[eid], self.dtype) if s is not None else t[eid].t()   # [2I, H]
                 self.w13.data[e].zero_()                 # (the padding included: the loader poisons fresh parameters)
                 self.w13.data[e, :I, :H].copy_(m[0::2][rows])
@@ -120,6 +135,30 @@ class GptOssMoE(FusedMoE):
                     self.b2.data[e].copy_(t[eid])
             else:
                 raise KeyError(kind)
+
+    def _pack(self, kind: str, w: torch.Tensor, scales: Optional[torch.Tensor], rows: slice) -> quant.MxWeight:
+        """One expert's matrix in the kernels' layout; this rank's rows (gate and up), or columns (down), of it."""
+        up = kind == "gate_up_proj"
+        dev = self.b13.device
+        if scales is None:
+            m = w.t()
+            m = torch.cat([m[0::2][rows], m[1::2][rows]]) if up else m[:, rows]
+            return mx_weight(m.to(device=dev, dtype=self.dtype).contiguous(), 2 if up else 1)
+        q, s = w.reshape(w.shape[0], -1), scales
+        if up:
+            q, s = (torch.cat([m[0::2][rows], m[1::2][rows]]) for m in (q, s))
+        else:
+            q, s = q[:, rows.start // 2:rows.stop // 2], s[:, rows.start // 32:rows.stop // 32]
+        return quant.pack_mx(q.to(dev).contiguous(), s.to(dev).contiguous(), halves=2 if up else 1)
+
+    def finalize_weights(self) -> None:
+        if not self.microscaled or self.mx13_qw is not None:
+            return
+        missing = [f"{kind}[{e}]" for kind, ws in self._blocks.items() for e, w in enumerate(ws) if w is None]
+        if missing:
+            raise RuntimeError(f"{len(missing)} expert matrices were not found in the checkpoint: {', '.join(missing[:8])}")
+        self._set_mx(self._blocks["gate_up_proj"], self._blocks["down_proj"])
+        self._blocks = {kind: [] for kind in self._blocks}
 
     # ------------------------------------------------------------------ compute
     def _act(self, h: torch.Tensor) -> torch.Tensor:
@@ -154,6 +193,9 @@ class GptOssMoE(FusedMoE):
 
     def forward(self, x: torch.Tensor, reduce: bool = True, staged: bool = False, deferred: bool = False):
         logits = self.gate(x)
+        if self.mx13_qw is not None:
+            out = self._experts_mx(x, logits, bias13=self.b13, bias2=self.b2, limit=self.limit, alpha=self.ALPHA)
+            return tensor_model_parallel_all_reduce(out) if reduce and self.tp > 1 else out
         tile_rows = self._expert_tile_rows(x)
         if tile_rows and x.dim() == 2 and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
             out = self._forward_fused_routing(x, logits, tile_rows)
@@ -200,7 +242,9 @@ class GptOssAttention(LlamaAttention):
 
 class GptOssDecoderLayer(LlamaDecoderLayer):
     def _make_attn(self, cfg: dict, layer_idx: int, dtype: torch.dtype, cos_sin: torch.Tensor) -> nn.Module:
-        return GptOssAttention(cfg, layer_idx, dtype, cos_sin)
+        spec = active_quant()
+        with quantized_linears(None if spec is not None and spec.method == "mxfp4" else spec):
+            return GptOssAttention(cfg, layer_idx, dtype, cos_sin)
 
     def _make_mlp(self, cfg: dict, dtype: torch.dtype) -> nn.Module:
         return GptOssMoE(cfg, dtype, _EP)
@@ -208,8 +252,9 @@ class GptOssDecoderLayer(LlamaDecoderLayer):
 
 class GptOssForCausalLM(LlamaForCausalLM):
     layer_cls = GptOssDecoderLayer
-    # the experts are widened to the model dtype at load whatever the checkpoint says about them
+    # the experts are widened to the model dtype at load whatever the checkpoint says about them, or stay microscaled (mxfp4)
     packed_quantization = False
+    mx_experts = True
 
     def __init__(self, vllm_config: VllmConfig):
         global _EP

@@ -518,10 +518,19 @@ class RMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(hidden_size, dtype=dtype), requires_grad=False)
         self.eps = eps
 
-    def forward(self, x, residual: Optional[torch.Tensor] = None):
+    def forward(self, x, residual: Optional[torch.Tensor] = None, rows8: bool = False):
         """``x`` may be a value its producer left unfinished - a projection's K-split partial sums
         (``layers.linear.PartialSums``) or the expert rows of a sparse block before their weighted sum
-        (``layers.moe.ExpertRows``): with a residual, the kernel that adds and normalises finishes it."""
+        (``layers.moe.ExpertRows``): with a residual, the kernel that adds and normalises finishes it.
+        ``rows8``: the normed rows leave as 8-bit microscaled ones (``ops.MxRows``), for a projection that takes them."""
+        if rows8:
+            if not isinstance(x, torch.Tensor):
+                if residual is not None and hasattr(x, "add_rms_norm_mx"):
+                    return x.add_rms_norm_mx(residual, self.weight, self.eps)
+                x = x.materialize()
+            if residual is None:
+                return ops.rms_norm_mx(x, self.weight, self.eps)
+            return ops.fused_add_rms_norm_mx(x, residual, self.weight, self.eps)
         if not isinstance(x, torch.Tensor):
             if residual is not None:
                 return x.add_rms_norm(residual, self.weight, self.eps)

@@ -38,7 +38,9 @@ class QuantSpec:
     ``nvfp4``: weight-only E2M1 with one e4m3 scale per 16 input columns and one
     fp32 scale per checkpoint matrix: ``weight_packed [out, in/2] uint8``,
     ``weight_scale [out, in/16] float8_e4m3fn``, ``weight_global_scale [1]``
-    (the reference image installs its fp4 kernels "for nvfp4", ``Dockerfile:5-6``)."""
+    (the reference image installs its fp4 kernels "for nvfp4", ``Dockerfile:5-6``).
+    ``mxfp4``: E2M1 weights with a power of two per 32 input columns, quantised once loaded, times 8-bit microscaled activations on the
+    scaled matrix instructions (``ops.mx_linear``)."""
     method: str = "awq"
     group_size: int = 128
     pack: int = 8
@@ -131,6 +133,13 @@ def awq_to_native(qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch.Ten
     return quant.pack_w4(q, z, scales.t().contiguous(), dtype)
 
 
+def mx_weight(w: torch.Tensor, halves: int = 1):
+    """Dense ``[out, in]`` -> 4-bit microscaled, in the kernels' layout (``ops.quant.pack_mx``)."""
+    from ...ops import quant
+    rows = ops.mx_quantize(w, 4)
+    return quant.pack_mx(rows.q, rows.s, halves=halves)
+
+
 class _LinearBase(nn.Module):
     """Dense ``weight [out, in]`` or, under ``quantized_linears``, the AWQ
     checkpoint triple which ``finalize_weights`` repacks once loading is done."""
@@ -145,14 +154,16 @@ class _LinearBase(nn.Module):
         self.register_buffer("weight_scale", None)
         self.register_buffer("alpha", None)
         self.register_buffer("dense_shadow", None)
+        self.register_buffer("mx_qw", None)
+        self.register_buffer("mx_ws", None)
         self.lora = None          # adapter slots, attached by lora.LoRAManager
         if spec is not None and spec.method == "nvfp4":
             assert in_local % 16 == 0, f"NVFP4 shard [{out_local} x {in_local}] splits a 16-column block"
             self.weight_packed = _tag(_param(out_local, in_local // 2, dtype=torch.uint8), 0, 1, 2)
             self.weight_block_scale = _tag(_param(out_local, in_local // 16, dtype=torch.float8_e4m3fn), 0, 1, 16)
             self.weight_alpha = _scalar_param(out_local)
-        elif spec is None or spec.method == "fp8":
-            # fp8: loaded in the checkpoint dtype, quantised per output channel in finalize_weights
+        elif spec is None or spec.method in ("fp8", "mxfp4"):
+            # fp8, mxfp4: loaded in the checkpoint dtype, quantised in finalize_weights
             self.weight = _tag(_param(out_local, in_local, dtype=dtype), 0)
         else:
             g = spec.group_size
@@ -172,7 +183,15 @@ class _LinearBase(nn.Module):
             self.bias.weight_loader = bias_loader or loader      # type: ignore[attr-defined]
 
     def finalize_weights(self) -> None:
-        if self.quant is None or self.qw is not None or self.weight_scale is not None:
+        if self.quant is None or self.qw is not None or self.weight_scale is not None or self.mx_qw is not None:
+            return
+        if self.quant.method == "mxfp4":
+            if self.in_local % 32 or self.out_local % 8:        # whole blocks, whole 16-byte pieces of a result's row
+                self.quant = None
+                return
+            w = mx_weight(self.weight.data)
+            del self.weight
+            self.mx_qw, self.mx_ws = w.qw, w.ws
             return
         if self.quant.method == "fp8":
             if self.in_local % 16 or self.out_local % 16:       # hipBLASLt fp8 alignment
@@ -206,6 +225,20 @@ class _LinearBase(nn.Module):
             from ..loader import awq_dequantize
             self.quant = None
             self.weight = nn.Parameter(awq_dequantize(qweight, qzeros, scales, self.dtype), requires_grad=False)
+
+    @property
+    def mx(self):
+        """The 4-bit microscaled weight, or None."""
+        return None if self.mx_qw is None else ops.MxWeight(self.mx_qw, self.mx_ws, self.out_local)
+
+    @property
+    def takes_rows8(self) -> bool:
+        """Whether the layer's input may come as 8-bit microscaled rows (``ops.MxRows``) from the kernel in front of it."""
+        return self.mx_qw is not None and self.lora is None
+
+    @property
+    def _dense16(self) -> bool:
+        return self.qw is None and self.weight_scale is None and self.mx_qw is None
 
     def pad_weight_rows(self, pad: int) -> bool:
         """Re-home a dense 16-bit GPU weight in a buffer whose rows are ``pad`` elements longer; the
@@ -250,6 +283,8 @@ class _LinearBase(nn.Module):
     def _base_matmul(self, x: torch.Tensor, bias: Optional[torch.Tensor],
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``out`` is a hint (dense 16-bit weights honour it): callers use what is returned."""
+        if self.mx_qw is not None:
+            return ops.mx_linear(x, self.mx, bias)
         if self.qw is not None:
             if self.alpha is not None:
                 return ops.fp4_linear(x, self.qw, self.sz, self.alpha, bias, self.dense_shadow)
@@ -338,13 +373,15 @@ class ColumnParallelLinear(_LinearBase):
             y = tensor_model_parallel_all_gather(y, dim=-1)
         return y
 
-    def forward_silu(self, x: torch.Tensor) -> Optional[torch.Tensor]:
+    def forward_silu(self, x: torch.Tensor, rows8: bool = False) -> Optional[torch.Tensor]:
         """``silu(gate) * up`` straight from ``x`` for a ``[gate ; up]`` layer when one kernel can do
-        it (dense 16-bit weights, large batch), else None: the caller falls back to ``forward`` plus
-        the activation."""
+        it (dense 16-bit weights, large batch; microscaled ones where the caller takes 8-bit rows: ``rows8``), else None: the caller
+        falls back to ``forward`` plus the activation."""
         if (self.qw is not None or self.weight_scale is not None or self.lora is not None or self.bias is not None
                 or self.gather_output or len(self.shard_sizes) != 2 or self.shard_sizes[0] != self.shard_sizes[1]):
             return None
+        if self.mx_qw is not None:          # (as 8-bit rows, for a projection that takes them)
+            return ops.mx_gate_up(x, self.mx) if rows8 and self.shard_sizes[0] % 128 == 0 else None
         return ops.gate_up_silu(x, self.weight)
 
 
@@ -398,14 +435,17 @@ class QKVParallelLinear(_LinearBase):
         """The packed ``[q | k | v]`` left as the fp32 K-split slabs of the short-batch kernels (dense
         16-bit or AWQ weights, no bias, no adapter) for the rotary + cache kernel to sum; None when the
         shape does not run split or the layer is not of that kind."""
-        if (self.weight_scale is not None or self.lora is not None or self.bias is not None
+        if self.mx_qw is not None and self.lora is None and self.bias is None and x.is_cuda and envs.VDAMD_FUSED_REDUCE_ROPE:
+            slabs = ops.mx_linear_partials(x, self.mx)
+            return None if slabs is None else PartialSums(slabs, x.dtype)
+        if (self.mx_qw is not None or self.weight_scale is not None or self.lora is not None or self.bias is not None
                 or self.alpha is not None or x.dim() != 2 or not x.is_cuda or not envs.VDAMD_FUSED_REDUCE_ROPE):
             return None
         slabs = ops.w4a16_partials(x, self.qw, self.sz) if self.qw is not None else ops.linear_partials(x, self.weight)
         return None if slabs is None else PartialSums(slabs, x.dtype)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if self.qw is None and self.weight_scale is None and self.lora is None and x.dim() == 2:
+        if self._dense16 and self.lora is None and x.dim() == 2:
             # large batches: the q columns alone tile the chip exactly, the k/v columns follow separately
             y = ops.linear_split(x, self.weight, self.q_size)
             if y is not None:
@@ -470,7 +510,7 @@ class RowParallelLinear(_LinearBase):
         fuse it with the following add + norm).  ``staged``: the partial sums are
         written where the TP group's next direct all-reduce reads its input."""
         out = None
-        if staged and self.tp > 1 and x.dim() == 2:
+        if staged and self.tp > 1 and self.mx_qw is None and x.dim() == 2:
             out = get_tp_group().stage_view((x.shape[0], self.out_local), x.dtype)
         # bias is added once (rank 0) so the all-reduce does not multiply it
         y = self._matmul(x, self.bias if self.tp_rank == 0 else None, out)
@@ -482,7 +522,10 @@ class RowParallelLinear(_LinearBase):
         """The product left as the fp32 K-split slabs of the short-batch kernels (an unsharded dense
         16-bit or AWQ layer, no bias, no adapter) for the add + RMSNorm that follows to sum; None when
         the shape does not run split or the layer is not of that kind."""
-        if (self.tp > 1 or self.weight_scale is not None or self.lora is not None or self.bias is not None
+        if self.mx_qw is not None and self.tp == 1 and self.lora is None and self.bias is None and x.is_cuda:
+            slabs = ops.mx_linear_partials(x, self.mx)
+            return None if slabs is None else PartialSums(slabs, x.dtype)
+        if (self.tp > 1 or self.mx_qw is not None or self.weight_scale is not None or self.lora is not None or self.bias is not None
                 or self.alpha is not None or x.dim() != 2 or not x.is_cuda):
             return None
         slabs = ops.w4a16_partials(x, self.qw, self.sz) if self.qw is not None else ops.linear_partials(x, self.weight)
@@ -492,7 +535,7 @@ class RowParallelLinear(_LinearBase):
         """``residual += x W^T`` in the GEMM's epilogue, for an unsharded dense 16-bit layer and a
         batch the large-batch kernel takes; False (nothing done) otherwise.  The add + RMSNorm that
         follows then only has to normalise ``residual``."""
-        if (self.tp > 1 or self.qw is not None or self.weight_scale is not None or self.lora is not None
+        if (self.tp > 1 or not self._dense16 or self.lora is not None
                 or self.bias is not None or x.dim() != 2):
             return False
         return ops.linear_add(x, self.weight, residual)
@@ -501,7 +544,7 @@ class RowParallelLinear(_LinearBase):
         """``forward(silu(gate) * up)`` for ``gate_up = [gate | up]``.  A dense 16-bit layer hands the
         pair to the GEMM, which forms the activation while it stages its operand (short batches on
         the weight-streaming kernel); every other layer runs the activation kernel first."""
-        if (self.qw is not None or self.weight_scale is not None or self.lora is not None or self.bias is not None
+        if (not self._dense16 or self.lora is not None or self.bias is not None
                 or gate_up.dim() != 2):
             return self.forward(ops.silu_and_mul(gate_up), reduce, staged)
         out = None
@@ -530,6 +573,9 @@ class PartialSums:
 
     def add_rms_norm(self, residual: torch.Tensor, weight: torch.Tensor, eps: float):
         return ops.reduce_add_rms_norm(self.slabs, residual, weight, eps)
+
+    def add_rms_norm_mx(self, residual: torch.Tensor, weight: torch.Tensor, eps: float):
+        return ops.reduce_add_rms_norm_mx(self.slabs, residual, weight, eps)
 
 
 def pad_vocab(vocab_size: int, tp: int, multiple: int = 64) -> int:

@@ -25,7 +25,7 @@ from ...parallel.state import (get_tensor_model_parallel_rank,
                                get_tensor_model_parallel_world_size,
                                tensor_model_parallel_all_reduce)
 from .linear import (ReplicatedLinear, _fill_scalar, active_quant, awq_to_native, divide, fp4_layout_ok,
-                     nvfp4_dequantize, w4_layout_ok)
+                     mx_weight, nvfp4_dequantize, w4_layout_ok)
 
 
 class ExpertRows:
@@ -70,6 +70,9 @@ class FusedMoE(nn.Module):
         self.hidden, self.dtype = hidden, dtype
         self.gate = ReplicatedLinear(hidden, num_experts, False, dtype, quant=False)   # router stays dense
         self.quant = active_quant()
+        # mxfp4: loaded dense, quantised in finalize_weights (here where the experts are this class' own)
+        self.microscaled = (self.quant is not None and self.quant.method == "mxfp4" and allocate_experts
+                            and type(self)._expert_mlp is FusedMoE._expert_mlp)
         if self.quant is not None and self.quant.method not in ("awq", "nvfp4"):
             self.quant = None           # fp8 covers the dense linears; experts stay in the model dtype
         E, I = self.local_experts, self.inter_local
@@ -79,6 +82,8 @@ class FusedMoE(nn.Module):
         self.register_buffer("sz2", None)
         self.register_buffer("alpha13", None)
         self.register_buffer("alpha2", None)
+        for name in ("mx13_qw", "mx13_ws", "mx2_qw", "mx2_ws"):
+            self.register_buffer(name, None)
 
         def param(*shape, dt=dtype, out_dim=0, pack=1, in_div=1, loader=None):
             p = nn.Parameter(torch.empty(*shape, dtype=dt), requires_grad=False)
@@ -145,6 +150,8 @@ class FusedMoE(nn.Module):
     def finalize_weights(self) -> None:
         """Repack the experts' AWQ shards into the 4-bit kernel layout (or
         dequantise them when a shard shape does not tile)."""
+        if self.microscaled and self.mx13_qw is None:
+            return self._finalize_mx()
         if self.quant is None or self.qw13 is not None:
             return
         E, I, H, g = self.local_experts, self.inter_local, self.hidden, self.quant.group_size
@@ -175,6 +182,28 @@ class FusedMoE(nn.Module):
             self.quant = None
             self.w13 = nn.Parameter(torch.stack(parts["13"]), requires_grad=False)
             self.w2 = nn.Parameter(torch.stack(parts["2"]), requires_grad=False)
+
+    def _finalize_mx(self) -> None:
+        if self.inter_local % 32 or self.hidden % 32 or self.num_experts > 512 or self.top_k > 16:
+            self.microscaled = False        # (whole blocks; what the slot sort takes)
+            return
+        self._set_mx([mx_weight(w, 2) for w in self.w13.data], [mx_weight(w) for w in self.w2.data])
+        del self.w13, self.w2
+
+    def _set_mx(self, w13: list, w2: list) -> None:
+        self.mx13_qw, self.mx13_ws = torch.stack([w.qw for w in w13]), torch.stack([w.ws for w in w13])
+        self.mx2_qw, self.mx2_ws = torch.stack([w.qw for w in w2]), torch.stack([w.ws for w in w2])
+
+    def _experts_mx(self, x: torch.Tensor, logits: torch.Tensor, **extra) -> torch.Tensor:
+        """The experts' products in microscaled floating point (``ops.mx_experts``), behind the router's choice."""
+        if not self.custom_routing and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
+            topw, topi = ops.moe_topk(logits, self.top_k, self.renormalize)
+        else:
+            topw, topi = self.route(logits.float())
+        weights = (ops.MxWeight(self.mx13_qw, self.mx13_ws, self.mx13_qw.shape[1] * 16),
+                   ops.MxWeight(self.mx2_qw, self.mx2_ws, self.hidden))
+        return ops.mx_experts(x, topw.float().contiguous(), topi.to(torch.int32).contiguous(), *weights, expert_start=self.expert_start,
+                              local_experts=self.local_experts if self.expert_parallel else -1, num_experts=self.num_experts, **extra)
 
     def _finalize_nvfp4(self) -> None:
         from ...ops import quant
@@ -315,6 +344,9 @@ class FusedMoE(nn.Module):
     def forward(self, x: torch.Tensor, reduce: bool = True, staged: bool = False, deferred: bool = False):
         # `deferred`: the caller feeds the result to an add + RMSNorm and accepts ``ExpertRows``
         # `staged` (write the partial sums where the next direct all-reduce reads) is a hint only
+        if self.mx13_qw is not None:
+            out = self._experts_mx(x, self.router_logits(x))
+            return tensor_model_parallel_all_reduce(out) if reduce and self.tp > 1 else out
         tile_rows = self._expert_tile_rows(x)
         logits = None
         if (tile_rows and not self.custom_routing and self.gate.bias is None

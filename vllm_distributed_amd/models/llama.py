@@ -114,7 +114,8 @@ class LlamaMLP(nn.Module):
         projection's K-split partial sums (``PartialSums``)."""
         if self.act != "silu":
             return self.down_proj(ops.act_and_mul(self.gate_up_proj(x), self.act), reduce, staged)
-        act = self.gate_up_proj.forward_silu(x)       # large batches: activation formed in the GEMM epilogue
+        # large batches: activation formed in the GEMM epilogue (microscaled layers: always, as 8-bit rows)
+        act = self.gate_up_proj.forward_silu(x, self.down_proj.takes_rows8)
         if act is not None:
             if residual is not None and self.down_proj.forward_add(act, residual):
                 return None
@@ -268,21 +269,24 @@ class LlamaDecoderLayer(nn.Module):
                 residual: Optional[torch.Tensor]) -> Tuple[Optional[torch.Tensor], torch.Tensor]:
         """``hidden`` None (in or out): the producing GEMM has already added its product into
         ``residual`` (large unsharded batches), so the norm that follows is a plain one."""
+        # projections with microscaled weights take their input as the 8-bit rows that the norm in front of them leaves
+        rows8 = {"rows8": True} if self._attn_partials and self.self_attn.qkv_proj.takes_rows8 else {}
         if residual is None:
             residual = hidden
-            hidden = self.input_layernorm(hidden)
+            hidden = self.input_layernorm(hidden, **rows8)
         elif hidden is None:
-            hidden = self.input_layernorm(residual)
+            hidden = self.input_layernorm(residual, **rows8)
         else:
-            hidden, residual = self.input_layernorm(hidden, residual)
+            hidden, residual = self.input_layernorm(hidden, residual, **rows8)
         if self._attn_partials:
             hidden = self.self_attn(positions, hidden, residual=residual, partials=True)
         else:
             hidden = self.self_attn(positions, hidden, residual=residual)
+        rows8 = {"rows8": True} if self._mlp_partials and self.mlp.gate_up_proj.takes_rows8 else {}
         if hidden is None:
-            hidden = self.post_attention_layernorm(residual)
+            hidden = self.post_attention_layernorm(residual, **rows8)
         else:
-            hidden, residual = self.post_attention_layernorm(hidden, residual)
+            hidden, residual = self.post_attention_layernorm(hidden, residual, **rows8)
         if self._mlp_partials:
             hidden = self.mlp(hidden, residual=residual, partials=True)
         elif self._mlp_deferred:
@@ -296,7 +300,7 @@ class LlamaDecoderLayer(nn.Module):
 
 class LlamaForCausalLM(nn.Module):
     layer_cls = LlamaDecoderLayer
-    # the linear layers are built under ``quantized_linears``: AWQ / NVFP4 / fp8 weights stay packed
+    # the linear layers are built under ``quantized_linears``: AWQ / NVFP4 / fp8 / mxfp4 weights stay packed
     packed_quantization = True
     # checkpoint name fragment -> (fused param fragment, shard id)
     stacked_params = [
@@ -325,7 +329,7 @@ class LlamaForCausalLM(nn.Module):
             self.embed_tokens = VocabParallelEmbedding(cfg["vocab_size"], cfg["hidden_size"], dtype,
                                                        out_scale=self.embedding_scale(cfg))
         spec = {"awq": QuantSpec("awq", mc.quant_group_size), "fp8": QuantSpec("fp8"),
-                "nvfp4": QuantSpec("nvfp4", 16, 1)}.get(mc.quantization)
+                "nvfp4": QuantSpec("nvfp4", 16, 1), "mxfp4": QuantSpec("mxfp4", 32, 1)}.get(mc.quantization)
         self.quant_method = spec.method if spec is not None else None
         with quantized_linears(spec):
             self.layers = nn.ModuleDict({

@@ -771,6 +771,9 @@ def load_model(vllm_config: VllmConfig, device: torch.device) -> torch.nn.Module
         # (those checkpoints still load with ``--quantization awq-dequant``: 16-bit weights, dense kernels)
         raise ValueError(f"{mc.architecture} has no packed 4-bit linear layers: quantization={mc.quantization!r} is "
                          f"supported for the Llama-shaped and expert-mixture families only")
+    if mc.quantization == "mxfp4" and not (getattr(cls, "packed_quantization", False) or getattr(cls, "mx_experts", False)):
+        raise ValueError(f"{mc.architecture} has no microscaled layers: quantization='mxfp4' is supported for the Llama-shaped and "
+                         f"expert-mixture families only")
     if mc.quantization == "fp8" and not getattr(cls, "packed_quantization", False):
         logger.warning("%s has no fp8 linear layers: weights are kept in %s", mc.architecture, mc.dtype)
     with torch.device(device):
@@ -806,6 +809,8 @@ def load_model(vllm_config: VllmConfig, device: torch.device) -> torch.nn.Module
             it = _gptq_as_awq(it, mc)
     with torch.no_grad():
         loaded = model.load_weights(_with_progress(it, "checkpoint tensors read"))
+        if mc.quantization == "mxfp4":
+            _check_filled(model, mc.model)       # (while the mark is there: blocks of 4-bit values do not carry it)
         mods = [m for m in model.modules() if getattr(m, "finalize_weights", None) is not None]
         for m in _with_progress(mods, "modules finalised"):      # repack quantised shards into the kernel layout
             m.finalize_weights()
@@ -901,4 +906,9 @@ def load_sharded_state(model: torch.nn.Module, path: str, rank: int, vllm_config
             for raw in ("qweight", "qzeros", "scales", "weight_packed", "weight_block_scale", "weight_alpha"):
                 if raw in mod._parameters:
                     del mod._parameters[raw]
+        if getattr(mod, "mx_qw", None) is not None:
+            mod._parameters.pop("weight", None)
+        if getattr(mod, "mx13_qw", None) is not None:
+            for raw in ("w13", "w2"):
+                mod._parameters.pop(raw, None)
     return n
