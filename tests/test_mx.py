@@ -5,7 +5,7 @@ import json
 import pytest
 import torch
 
-import mx_oracle as oracle
+from tests import mx_oracle as oracle
 from vllm_distributed_amd import LLM, SamplingParams, ops
 from vllm_distributed_amd.config import ModelConfig
 from vllm_distributed_amd.ops import quant

@@ -311,6 +311,26 @@ def make_experts(e, n, k, halves=1):
     return w, torch.stack([p[2] for p in parts])
 
 
+def expert_block(xv, topw, topi, v13, v2, b13, b2, limit):
+    """The sparse block of rows ``xv`` in 64 bits (matrices as numbers, ``[E, ..]``), and how far a bfloat16 result may be from it."""
+    want = torch.zeros(xv.shape[0], v2.shape[1], dtype=torch.float64)
+    bound = torch.zeros_like(want)
+    for j in range(len(v2)):
+        r, c = (topi == j).nonzero(as_tuple=True)
+        if not len(r):
+            continue
+        v, slack = gated_slack(xv[r], v13[j], None if b13 is None else b13[j].cpu(), limit)
+        a = oracle.blocks(v, 8)[2]
+        z = a @ v2[j].T + (0 if b2 is None else b2[j].cpu().double())
+        # an activation beside the middle of two elements may go to the other: a step of 2^-3 of it (2^-9 of its scale where subnormal)
+        flips = torch.maximum(2.0 ** -3 * v.abs(), 2.0 ** -18 * v.abs().reshape(len(r), -1, 32).amax(-1).repeat_interleave(32, 1)) + slack
+        near = oracle.blocks(v + slack, 8)[2] != oracle.blocks(v - slack, 8)[2]
+        d = (flips * near) @ v2[j].abs().T + SUM * (a.abs() @ v2[j].abs().T)
+        want.index_add_(0, r, z * topw[r, c].double().unsqueeze(1))
+        bound.index_add_(0, r, (d + 2.0 ** -20 * z.abs()) * topw[r, c].double().unsqueeze(1))      # (up to four 32-bit products and sums)
+    return want, bound + 2.0 ** -8 * (want.abs() + bound)
+
+
 @pytest.mark.parametrize("t,e,k,h,inter,limit", [(1, 8, 2, 128, 128, 0.0), (16, 128, 4, 288, 160, 7.0), (9, 4, 4, 160, 128, 7.0),
                                                  (70, 8, 2, 256, 384, 0.0), (40, 4, 2, 416, 160, 7.0), (150, 4, 2, 160, 288, 7.0), (300, 5, 3, 96, 96, 7.0), (1200, 4, 2, 256, 128, 0.0), (513, 3, 2, 160, 416, 7.0)])
 def test_experts(t, e, k, h, inter, limit):
@@ -326,21 +346,7 @@ def test_experts(t, e, k, h, inter, limit):
     topw = torch.rand(t, k)
     y = ops.mx_experts(x.cuda(), topw.cuda(), topi.cuda(), w13, w2, None if b13 is None else quant.pad_mx_bias(b13, 2).cuda(),
                        None if b2 is None else b2.cuda(), limit=limit)
-    xv, want, bound = oracle.blocks(x, 8)[2], torch.zeros(t, h, dtype=torch.float64), torch.zeros(t, h, dtype=torch.float64)
-    for j in range(e):
-        r, c = (topi == j).nonzero(as_tuple=True)
-        if not len(r):
-            continue
-        v, slack = gated_slack(xv[r], v13[j], None if b13 is None else b13[j], limit)
-        a = oracle.blocks(v, 8)[2]
-        z = a @ v2[j].T + (0 if b2 is None else b2[j].double())
-        # an activation beside the middle of two elements may go to the other: a step of 2^-3 of it (2^-9 of its scale where subnormal)
-        flips = torch.maximum(2.0 ** -3 * v.abs(), 2.0 ** -18 * v.abs().reshape(len(r), -1, 32).amax(-1).repeat_interleave(32, 1)) + slack
-        near = oracle.blocks(v + slack, 8)[2] != oracle.blocks(v - slack, 8)[2]
-        d = (flips * near) @ v2[j].abs().T + SUM * (a.abs() @ v2[j].abs().T)
-        want.index_add_(0, r, z * topw[r, c].double().unsqueeze(1))
-        bound.index_add_(0, r, (d + 2.0 ** -20 * z.abs()) * topw[r, c].double().unsqueeze(1))      # (up to four 32-bit products and sums)
-    bound = bound + 2.0 ** -8 * (want.abs() + bound)
+    want, bound = expert_block(oracle.blocks(x, 8)[2], topw, topi, v13, v2, b13, b2, limit)
     off = (y.cpu().double() - want).abs()
     assert (off <= bound).all(), f"worst {(off / bound).max():.3g} of the bound"
     assert off.norm() <= 2.0 ** -6 * want.norm()
