@@ -117,7 +117,7 @@ def _parse():
     ap.add_argument("--ttft-requests", type=int, default=5)
     ap.add_argument("--dtype", type=str, default="bfloat16")
     ap.add_argument("--enforce-eager", action="store_true")
-    ap.add_argument("--quantization", type=str, default=None, choices=[None, "fp8", "awq", "nvfp4"],
+    ap.add_argument("--quantization", type=str, default=None, choices=[None, "fp8", "awq", "nvfp4", "mxfp4"],
                     help="NOT the headline configuration (that is bf16): reduced-precision linears")
     ap.add_argument("--kv-cache-dtype", type=str, default="auto",
                     help="NOT the headline configuration (that is bf16): e.g. fp8 KV cache")
