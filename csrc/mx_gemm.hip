@@ -607,49 +607,63 @@ int mx_big(const MxArgs& a, hipStream_t st) {
   return 0;
 }
 
-// Between: rows enough that x is worth sharing, too few to fill the chip with 256-row tiles.  A workgroup has 16 MT rows and 4 NT column
-// tiles, its four waves NT of them each and all of the rows; K in steps of 128, split over the grid.  x and the weights of S steps are in
-// LDS or on their way to it, straight from memory: the loads of the step that is S - 1 ahead go out while one is multiplied, so
-// (S - 1) (2 MT + 4 NT) KiB a workgroup are in flight, and the bytes of the weights are the time until the matrix cores are.
-// A step is one barrier: behind it every wave's loads of the step are there and every wave has read the step before.  (Reading the next
-// step's fragments while this one's are multiplied takes a step off what is in flight, and was slower at every size: 8192 x 28672 by
+// Between: rows enough that x is worth sharing, too few to fill the chip with 256-row tiles.  A workgroup has 16 MT WM rows and 4 NT column
+// tiles, a wave NT of them and 16 MT of the rows; K in steps of 128, split over the grid.  x and the weights of S steps are in LDS or on
+// their way to it, straight from memory: the loads of the step that is S - 1 ahead go out while one is multiplied, so
+// (S - 1) (2 MT WM + 4 NT) KiB a workgroup are in flight, and the bytes of the weights are the time until the matrix cores are.
+// WM 1: a step is one barrier; behind it every wave's loads of the step are there and every wave has read the step before.  (Reading the
+// next step's fragments while this one's are multiplied takes a step off what is in flight, and was slower at every size: 8192 x 28672 by
 // 100 rows 43 -> 53 us.)
+// WM 2: 128 rows, two waves to a SIMD; those of the second half of the rows run half a step behind, so that the matrix cores multiply for
+// the one while the other reads LDS: a step is two barriers, a wave reads in front of one and multiplies behind it.  Its loads go out
+// between its products: the first half's of the step that is S - 1 ahead (the second half still reads this step), the second's of the
+// one that is S ahead, into the buffer that both are done with.  256 rows of 28672 into 8192 in four parts: 75 us with both halves in step,
+// 68 with the halves apart, 66 with the loads between the products; 1024 of 8192 into 8192 69, 64, 60 (of which 42 are the instructions').
 // Scales come 16 bytes a row (four steps) at a time, with the first step of each four, into sets of their own.
 // MX_GLU: NT 4, a wave's tiles are two of the gate and the same two of the up half - a block of 32 columns.
-template <int MT, int NT> struct MxRing {
-  static constexpr int X = MT * 2048, STEP = X + NT * 4096;               // bytes of a step
-  static constexpr int XR = MT < 4 ? 64 : 16 * MT, SCALES = XR * 16 + NT * 1024;      // rows whose scales are loaded, bytes of a set
+template <int MT, int NT, int WM> struct MxRing {
+  static constexpr int X = WM * MT * 2048, STEP = X + NT * 4096;          // bytes of a step
+  static constexpr int XR = WM * (MT < 4 ? 64 : 16 * MT), SCALES = XR * 16 + NT * 1024;      // rows whose scales are loaded, bytes of a set
   // the sets that S steps under way and the one that is multiplied may touch
   static constexpr int sets(int steps) { return (steps + 2) / 4 + 1; }
   static constexpr int bytes(int steps) { return steps * STEP + sets(steps) * SCALES; }
   static constexpr int fit(int lds) { int n = 2; while (n < 8 && bytes(n + 1) <= lds) ++n; return n; }
 };
-template <typename T, int MT, int NT, int EPI, int S>
-__global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
+template <typename T, int MT, int NT, int WM, int EPI, int S>
+__global__ __launch_bounds__(256 * WM) void mx_ring_kernel(const MxArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using R = MxRing<MT, NT>;
-  constexpr int SCB = R::SCALES, SETS = R::sets(S);
+  using R = MxRing<MT, NT, WM>;
+  constexpr int ROWS = 16 * MT * WM, WP = NT / WM, SCB = R::SCALES, SETS = R::sets(S);
   __shared__ __attribute__((aligned(1024))) unsigned char smem[R::bytes(S)];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wid & 3, wm = wid >> 2;                       // this wave's columns, rows
   const int r = lane & 15, q = lane >> 4;
   const int KB = a.KB, SS = (KB + 3) >> 2, ntiles = (a.N + 15) >> 4, half = ntiles >> 1;
-  int row0 = blockIdx.x * (16 * MT), end = a.M, group = 0;
+  int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
+  if (a.tiles == nullptr && ((gridDim.y * gridDim.z) & 7) == 0) {      // row tiles of the same weights on one of the eight dies, in turn
+    const unsigned l = bx + gridDim.x * (by + gridDim.y * bz), u = l / (8 * gridDim.x) * 8 + (l & 7);
+    bx = (l >> 3) % gridDim.x;
+    by = u % gridDim.y;
+    bz = u / gridDim.y;
+  }
+  int row0 = bx * ROWS, end = a.M, group = 0;
   if (a.tiles != nullptr) {
-    const int* d = a.tiles + 3 * blockIdx.x;
+    const int* d = a.tiles + 3 * bx;
     const int rows = __builtin_amdgcn_readfirstlane(d[2]);
     if (rows <= 0) return;
     group = min(max(__builtin_amdgcn_readfirstlane(d[0]), 0), a.groups - 1);
     row0 = min(max(__builtin_amdgcn_readfirstlane(d[1]), 0), a.M - 1);
-    end = min(a.M, row0 + min(rows, 16 * MT));
+    end = min(a.M, row0 + min(rows, ROWS));
   }
   // this workgroup's steps
-  const int lo = (int)((long)KB * blockIdx.z / a.ksplit), hi = (int)((long)KB * (blockIdx.z + 1) / a.ksplit);
-  int nt0[NT];                                                 // this wave's column tiles
+  const int lo = (int)((long)KB * bz / a.ksplit), hi = (int)((long)KB * (bz + 1) / a.ksplit);
+  auto column_tile = [&](int j) {                              // behind tile j of the workgroup's 4 NT: NT of each wave
+    if (EPI == MX_GLU) return 2 * (4 * by + j / NT) + (j & 1) + ((j % NT) >> 1) * half;
+    return 4 * NT * by + j;
+  };
+  int ld0[WP];                                                 // those that this wave loads
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (EPI == MX_GLU) nt0[t] = 2 * (4 * (int)blockIdx.y + wid) + (t & 1) + (t >> 1) * half;
-    else nt0[t] = (4 * (int)blockIdx.y + wid) * NT + t;
-  }
+  for (int t = 0; t < WP; ++t) ld0[t] = column_tile(wid * WP + t);
 
   // ---- staging.  Rows past the end, tiles past the last come as zeros from outside their descriptors
   const unsigned wbytes = (unsigned)((long)ntiles * KB * 1024), sbytes = (unsigned)((long)ntiles * SS * 256);
@@ -659,8 +673,8 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
   const auto wsr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.ws + (long)group * sbytes), 0, (int)sbytes, 0x00020000);
   const unsigned ldq = (unsigned)a.ldq;
   // x: MT / 2 pieces of eight rows a wave (MT 2: one); a row's 16-byte slots XOR-ed with (row >> 1) & 7
-  constexpr int XP = MT / 2;
-  unsigned xoff[XP], soff[R::XR / 64];
+  constexpr int XP = MT / 2, XS = R::XR / (64 * WM);
+  unsigned xoff[XP], soff[XS];
   auto row_of = [&](int m) {                                   // of x behind row m of this workgroup
     int row = min(row0 + m, end - 1);
     if (a.src != nullptr) row = min(max(a.src[row], 0), a.x_rows - 1);
@@ -673,28 +687,29 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
   }
   // scales of x: 64 lanes x 4 bytes, 16 rows of 16 bytes each; MT < 4: the last rows again
 #pragma unroll
-  for (int i = 0; i < R::XR / 64; ++i) soff[i] = row_of(min(16 * (R::XR / 64 * wid + i) + (lane >> 2), 16 * MT - 1)) * (unsigned)a.lds + 4 * (lane & 3);
+  for (int i = 0; i < XS; ++i) soff[i] = row_of(min(16 * (XS * wid + i) + (lane >> 2), ROWS - 1)) * (unsigned)a.lds + 4 * (lane & 3);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (loads of src: nothing of them among the counted ones)
-  constexpr int PER = XP + NT;                                 // loads of a wave and step, without scales
-  auto stage = [&](int k, int buf) {
-    unsigned char* const to = smem + buf * R::STEP;
-#pragma unroll
-    for (int i = 0; i < XP; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mx_lds_void*)(to + (XP * wid + i) * 1024), 16, xoff[i], k * 128, 0, 0);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (mx_lds_void*)(to + R::X + (wid * NT + t) * 1024), 16,
-                                               16u * lane + (unsigned)nt0[t] * (unsigned)(KB * 1024), k * 1024, 0, 0);
+  constexpr int PER = XP + WP;                                 // loads of a wave and step, without scales
+  int sbuf = 0, sset = 0;                                      // where the next step's and the next set's loads go
+  auto stage = [&](int k, int p) {                             // load p of PER of step k; behind the last step: zeros, read by nobody
+    unsigned char* const to = smem + sbuf * R::STEP;
+    const unsigned off = __builtin_amdgcn_readfirstlane(k < hi ? 0u : 0xfffffff0u);
+    const int at = __builtin_amdgcn_readfirstlane(min(k, hi - 1));
+    if (p < XP)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (mx_lds_void*)(to + (XP * wid + p) * 1024), 16, xoff[p] | off, at * 128, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (mx_lds_void*)(to + R::X + (wid * WP + p - XP) * 1024), 16,
+                                               (16u * lane + (unsigned)ld0[p - XP] * (unsigned)(KB * 1024)) | off, at * 1024, 0, 0);
   };
   auto stage_scales = [&](int ss, int set) {
     unsigned char* const to = smem + S * R::STEP + set * SCB;
 #pragma unroll
-    for (int i = 0; i < R::XR / 64; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(xsr, (mx_lds_void*)(to + (R::XR / 64 * wid + i) * 256), 4, soff[i], ss * 16, 0, 0);
+    for (int i = 0; i < XS; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xsr, (mx_lds_void*)(to + (XS * wid + i) * 256), 4, soff[i], ss * 16, 0, 0);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mx_lds_void*)(to + R::XR * 16 + (wid * NT + t) * 256), 4,
-                                               4u * lane + (unsigned)nt0[t] * (unsigned)(SS * 256), ss * 256, 0, 0);
+    for (int t = 0; t < WP; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (mx_lds_void*)(to + R::XR * 16 + (wid * WP + t) * 256), 4,
+                                               4u * lane + (unsigned)ld0[t] * (unsigned)(SS * 256), ss * 256, 0, 0);
   };
 
   f32x4 acc[NT][MT];
@@ -705,56 +720,99 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
   const int swz = (r >> 1) & 7, so0 = (q ^ swz) << 4, so1 = ((4 + q) ^ swz) << 4;
   // set of four steps ss: (ss - first) mod SETS; a step's buffer: (k - lo) mod S
   const int first = lo >> 2;
-  int sbuf = 0, sset = 0;                                      // where the next step's and the next set's loads go
-  auto issue = [&](int k) {                                    // everything of step k
-    if (k == lo || (k & 3) == 0) {
+  auto issue_scales = [&](int k) {
+    if (k < hi && (k == lo || (k & 3) == 0)) {
       stage_scales(k >> 2, sset);
       sset = sset + 1 == SETS ? 0 : sset + 1;
     }
-    stage(k, sbuf);
-    sbuf = sbuf + 1 == S ? 0 : sbuf + 1;
   };
-  for (int k = lo; k < min(lo + S - 1, hi); ++k) issue(k);
+  // Step k in n parts, this is part i.  (A unit takes a load in 16 cycles: those of all waves in a row, in front of their reads of LDS, hold
+  // these up; between the products they do not.)
+  auto issue = [&](int k, int i, int n) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (p * n / PER == i) stage(k, p);
+    if (i == n - 1) sbuf = sbuf + 1 == S ? 0 : sbuf + 1;
+  };
+  const int ahead = S - 1 + wm;
+  for (int k = lo; k < lo + ahead; ++k) {
+    issue_scales(k);
+    issue(k, 0, 1);
+  }
   int buf = 0, set = 0;
-  for (int k = lo; k < hi; ++k) {
+  // at most the S - 2 steps behind the one that is read next are in flight (scales among them make the count stricter)
+  auto arrived = []() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * PER) : "memory"); };
+  auto meet = []() {
     __builtin_amdgcn_sched_barrier(0);
-    // at most the S - 2 steps behind this one are in flight (scales among them make the count stricter); near the end fewer: all
-    if (k + S - 2 < hi) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * PER) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (k + S - 1 < hi) issue(k + S - 1);
-    const unsigned char* const at = smem + buf * R::STEP;
-    const unsigned char* const sc = smem + S * R::STEP + set * SCB;
-    mx_u32x4 w[NT];
-    uint32_t sw[NT];
+  };
+  auto next = [&](int k) {
+    buf = buf + 1 == S ? 0 : buf + 1;
+    if ((k & 3) == 3) set = set + 1 == SETS ? 0 : set + 1;
+  };
+  mx_u32x4 w[NT];
+  uint32_t sw[NT];
+  auto read_weights = [&](int k) {
+    const unsigned char* const at = smem + buf * R::STEP + R::X + wn * NT * 1024 + lane * 16;
+    const unsigned char* const sc = smem + S * R::STEP + set * SCB + R::XR * 16 + wn * NT * 256 + lane * 4 + (k & 3);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      w[t] = *reinterpret_cast<const mx_u32x4*>(at + R::X + (wid * NT + t) * 1024 + lane * 16);
-      sw[t] = sc[R::XR * 16 + (wid * NT + t) * 256 + lane * 4 + (k & 3)];
+      w[t] = *reinterpret_cast<const mx_u32x4*>(at + t * 1024);
+      sw[t] = sc[t * 256];
+    }
+  };
+  auto row = [&](int k, int i, mx_i32x8& x, uint32_t& sx) {
+    const int m = 16 * (MT * wm + i) + r;
+    const unsigned char* const at = smem + buf * R::STEP + m * 128;
+    x = mx_fragment(at + so0, at + so1);
+    sx = smem[S * R::STEP + set * SCB + m * 16 + 4 * (k & 3) + q];
+  };
+  mx_i32x8 x[MT];
+  uint32_t sx[MT];
+  if (wm == 1) {
+    arrived();
+    meet();
+  }
+  for (int k = lo; k < hi; ++k) {
+    if (wm == 0) arrived();
+    meet();
+    issue_scales(k + ahead);
+    read_weights(k);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) row(k, i, x[i], sx[i]);
+    next(k);
+    if constexpr (WM == 2) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      arrived();
+      meet();
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const unsigned char* const p = at + (16 * i + r) * 128;
-      const mx_i32x8 x = mx_fragment(p + so0, p + so1);
-      const uint32_t sx = sc[(16 * i + r) * 16 + 4 * (k & 3) + q];
+      issue(k + ahead, i, MT);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t][i] = mx_mfma(w[t], x, acc[t][i], sw[t], sx);
+      for (int t = 0; t < NT; ++t) acc[t][i] = mx_mfma(w[t], x[i], acc[t][i], sw[t], sx[i]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    buf = buf + 1 == S ? 0 : buf + 1;
-    if ((k & 3) == 3) set = set + 1 == SETS ? 0 : set + 1;
+    if constexpr (WM == 2)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) asm volatile("" : "+v"(acc[t][i]));    // (multiplied here, not behind the next barrier)
   }
+  if (WM == 2 && wm == 0) meet();
 
   // ---- lane (r, q): columns 4 q .. + 3 of tile t, row 16 i + r
   if constexpr (EPI == MX_GLU) {
-    const int n0 = 32 * (4 * blockIdx.y + wid), n1 = n0 + (a.N >> 1);
+    const int n0 = 32 * (4 * by + wn), n1 = n0 + (a.N >> 1);
     if (n0 >= a.N >> 1) return;
     float b0[2][4], b1[2][4];
     mx_bias<T>(b0, a.bias, (long)group * a.N, n0, a.N, q);
     mx_bias<T>(b1, a.bias, (long)group * a.N, n1, a.N, q);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int m = row0 + 16 * i + r;
+      const int m = row0 + 16 * (MT * wm + i) + r;
       float v[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -766,7 +824,7 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
     const T* bias = a.bias == nullptr ? nullptr : (const T*)a.bias + (long)group * a.N;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int n = 16 * nt0[t] + 4 * q;
+      const int n = 16 * column_tile(wn * NT + t) + 4 * q;
       if (n >= a.N) continue;
       f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
       if (bias != nullptr)
@@ -774,10 +832,10 @@ __global__ __launch_bounds__(256) void mx_ring_kernel(const MxArgs a) {
         for (int e = 0; e < 4; ++e) b[e] = (float)bias[n + e];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const int m = row0 + 16 * i + r;
+        const int m = row0 + 16 * (MT * wm + i) + r;
         if (m >= end) continue;
         if constexpr (EPI == MX_SLAB) {
-          *reinterpret_cast<f32x4*>(a.partial + ((long)blockIdx.z * a.M + m) * a.N + n) = acc[t][i] + b;
+          *reinterpret_cast<f32x4*>(a.partial + ((long)bz * a.M + m) * a.N + n) = acc[t][i] + b;
         } else {
           typename Vec4<T>::type o;
 #pragma unroll
@@ -906,28 +964,26 @@ int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
   return 0;
 }
 
-// row_tiles 2, 4 or 8, n_tiles 2 (MX_GLU: 4), waves 1.  As many steps as fit half of a unit's LDS: two workgroups a unit hide each other's
-// barriers (twice the steps in one workgroup's: 8192 x 28672 by 48 rows 31 -> 35 us, 6144 x 4096 by 411 25.3 -> 25.7)
-template <typename T, int EPI, int MT, int NT>
+// row_tiles 2 or 4, n_tiles 2 (MX_GLU: 4); 8 and 4.  As many steps as fit half of a unit's LDS: two workgroups a unit hide each other's
+// barriers (twice the steps in one workgroup's: 8192 x 28672 by 48 rows 31 -> 35 us, 6144 x 4096 by 411 25.3 -> 25.7); 128 rows: all of it
+template <typename T, int EPI, int MT, int NT, int WM>
 int mx_ring_go(const MxArgs& a, hipStream_t st) {
-  constexpr int S = MxRing<MT, NT>::fit(MT * NT <= 16 ? 80 * 1024 : 158 * 1024);
+  constexpr int S = MxRing<MT, NT, WM>::fit(MT * NT * WM <= 16 ? 80 * 1024 : 158 * 1024), ROWS = 16 * MT * WM;
   const int ntiles = (a.N + 15) / 16, per = 4 * NT;
-  dim3 grid(a.tiles != nullptr ? a.num_tiles : (a.M + 16 * MT - 1) / (16 * MT), (ntiles + per - 1) / per, a.ksplit);
-  if (grid.y > 65535 || grid.z > 65535) return -7;
-  mx_ring_kernel<T, MT, NT, EPI, S><<<grid, 256, 0, st>>>(a);
+  dim3 grid(a.tiles != nullptr ? a.num_tiles : (a.M + ROWS - 1) / ROWS, (ntiles + per - 1) / per, a.ksplit);
+  if (grid.y > 65535 || grid.z > 65535 || (long)grid.x * grid.y * grid.z >= (1L << 31)) return -7;
+  mx_ring_kernel<T, MT, NT, WM, EPI, S><<<grid, 256 * WM, 0, st>>>(a);
   HIP_LAUNCH_CHECK();
   return 0;
 }
 template <typename T, int EPI>
 int mx_ring(const MxArgs& a, int mt, int nt, hipStream_t st) {
   const long lim = (1L << 32) - 64;
+  if (a.x16 != nullptr || (long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim) return -8;
   constexpr int NT = EPI == MX_GLU ? 4 : 2;
-  if (a.x16 != nullptr || (long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim || nt != NT) return -8;
-  switch (mt) {
-    case 2: return mx_ring_go<T, EPI, 2, NT>(a, st);
-    case 4: return mx_ring_go<T, EPI, 4, NT>(a, st);
-    case 8: return mx_ring_go<T, EPI, 8, NT>(a, st);
-  }
+  if (mt == 2 && nt == NT) return mx_ring_go<T, EPI, 2, NT, 1>(a, st);
+  if (mt == 4 && nt == NT) return mx_ring_go<T, EPI, 4, NT, 1>(a, st);
+  if (mt == 8 && nt == 4) return mx_ring_go<T, EPI, 4, 4, 2>(a, st);
   return -6;
 }
 
@@ -972,7 +1028,8 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t
 // 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales (ksplit > 1: through partial); limit 0: SiLU.
 // tiles [num_tiles][3] (matrix, first row, rows; ksplit 1) or null; src [M] or null: the row of x behind each row.
 // shape: 16-row tiles a workgroup takes (of `tiles` at most 16 times as many rows each) + 256 times its 16-column tiles + 65536 times its
-// waves for the streaming kernel (mx_stream);  row tiles 2, 4 or 8 + 256 times 2 (4 where epi is 2 and ksplit 1) + 65536: the ring of LDS;
+// waves for the streaming kernel (mx_stream);  row tiles 2 or 4 + 256 times 2 (4 where epi is 2 and ksplit 1), or 8 + 256 times 4, + 65536:
+// the ring of LDS;
 // 16: the kernel of 256-row tiles (ksplit 1, src null).  The last two: x_rows ldq and a matrix's bytes below 2^32, lds a multiple of 16.
 VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* partial, const void* xq, long ldq, const void* xs, long lds,
                             int x_rows, const void* x16, long ldx, int K, const void* qw, const void* ws, const void* bias, int M, int N,

@@ -242,6 +242,25 @@ def test_linear_rows_do_not_mix(m):
     assert y[:, 37].isnan().all() and torch.equal(y[:, cols.cuda()], clean[:, cols.cuda()])
 
 
+@pytest.mark.parametrize("mt,nt,ksplit", [(2, 2, 1), (2, 2, 2), (4, 2, 1), (4, 2, 3), (8, 4, 1), (8, 4, 3), (2, 4, 1)])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 544), (130, 1000, 544), (257, 264, 2880), (700, 2560, 1184)])
+def test_every_shape_of_the_ring(m, n, k, mt, nt, ksplit, monkeypatch):
+    """Shapes of the launch that the plan keeps for other sizes, at ragged ones: the answer is the same."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    x, b = rows(m, k), torch.randn(n).to(torch.bfloat16)
+    w, wv = make(n, k)
+    xr = ops.mx_quantize(x.cuda())
+    monkeypatch.setattr(hip, "mx_plan", lambda *a: (hip._mx_shape(mt, nt, 1), ksplit))
+    if mt == 8 or nt == 2:
+        check_product(ops.mx_linear(xr, w, b.cuda()), oracle.blocks(x, 8)[2], wv, torch.bfloat16, b)
+    if nt == 4 and ksplit == 1:
+        w, wv = make(256 * (n // 256 + 1), k, halves=2, spread=1)
+        xr = ops.mx_quantize((x.float() / k ** 0.5).to(torch.bfloat16).cuda())
+        v, slack = gated_slack(ops.mx_dequantize(xr, torch.float32).cpu().double(), wv, None, 0.0)
+        check_rows(ops.mx_gate_up(xr, w), v, slack)
+
+
 @pytest.mark.parametrize("m,n,k", [(40, 512, 4096), (64, 2880, 4096)])
 def test_partials_and_the_norm_behind_them(m, n, k):
     from vllm_distributed_amd import ops
@@ -332,6 +351,7 @@ def expert_block(xv, topw, topi, v13, v2, b13, b2, limit):
 
 
 @pytest.mark.parametrize("t,e,k,h,inter,limit", [(1, 8, 2, 128, 128, 0.0), (16, 128, 4, 288, 160, 7.0), (9, 4, 4, 160, 128, 7.0),
+                                                 (64, 4, 2, 416, 160, 7.0), (200, 4, 2, 160, 288, 7.0), (220, 4, 2, 288, 160, 0.0),
                                                  (70, 8, 2, 256, 384, 0.0), (40, 4, 2, 416, 160, 7.0), (150, 4, 2, 160, 288, 7.0), (300, 5, 3, 96, 96, 7.0), (1200, 4, 2, 256, 128, 0.0), (513, 3, 2, 160, 416, 7.0)])
 def test_experts(t, e, k, h, inter, limit):
     from vllm_distributed_amd import ops

@@ -615,7 +615,7 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
         raise ValueError(f"{e_local} and {weight2.qw.shape[0]} expert matrices, {local_experts} local experts")
     if _mx_hip(x.payload if isinstance(x, MxRows) else x, dtype) and t:
         tile_rows = _hip.mx_tile_rows(t * k, total)
-        if tile_rows == 256 and not (_hip.mx_sorted_ok(t * k, weight13) and _hip.mx_sorted_ok(t * k, weight2)):
+        if tile_rows > 64 and not (_hip.mx_sorted_ok(t * k, weight13) and _hip.mx_sorted_ok(t * k, weight2)):
             tile_rows = 64
         src_row, inv, tiles = moe_align_fused(topi, total, tile_rows, expert_start, local_experts)
         if tile_rows == 256:          # (large tiles read their rows in order: quantised, or gathered, into it)

@@ -2559,21 +2559,22 @@ def _mx_shape(mt: int, nt: int, waves: int) -> int:
 
 
 # us of a step of the ring kernel's workgroups by (16-row tiles, column tiles of a wave): of one alone on a unit, of each that shares one;
-# fitted with the other constants of _mx_estimate to 16 shapes of 1000 to 57344 columns and 1024 to 28672 of reduction by 8 to 2048 rows
-# (the choice is within 2 % of the best of them on average, 28 % at worst)
-_MX_RING = {(2, 2): (0.30, 0.31), (4, 2): (0.49, 0.29), (8, 2): (0.96, 0.77), (2, 4): (0.39, 0.41), (4, 4): (0.55, 0.46)}
+# fitted with the other constants of _mx_estimate to 18 shapes of 640 to 57344 columns and 1024 to 28672 of reduction by 8 to 2048 rows
+# (the choice is within 1 % of the best of them on average, 16 % at worst)
+_MX_RING = {(2, 2): (0.23, 0.26), (4, 2): (0.42, 0.32), (2, 4): (0.47, 0.36), (8, 4): (0.68, 0.82)}
 
 
 def _mx_estimate(m: int, n: int, kb: int, mt: int, nt: int, ksplit: int) -> float:
     """Expected us of a product; ``mt`` ``MX_BIG``: 256-row tiles, whose steps slow down as they fill the chip."""
     if mt == MX_BIG:
         tiles = -(-m // 256) * -(-n // 256)
-        return -(-tiles // 256) * (kb * (1.02 + 0.3 * min(1.0, max(0.0, (tiles - 128) / 128))) + 6)
+        return -(-tiles // 256) * (kb * (1.0 + 0.22 * min(1.0, max(0.0, (tiles - 128) / 128))) + 5.4)
     load = -(-n // (64 * nt)) * -(-m // (16 * mt)) * ksplit / 256
     alone, shared = _MX_RING[mt, nt]
-    t = 3.5 + -(-kb // ksplit) * max(alone, shared * (math.ceil(load) if load <= 2 else load + 0.5))
+    # (workgroups of 128 rows have a unit to themselves: in rounds)
+    t = 4.7 + -(-kb // ksplit) * max(alone, shared * (math.ceil(load) if load <= 2 or mt == 8 else load + 0.5))
     t = max(t, n * kb * 128 * 17 / 32 / 4.9e6 + 3)
-    return t if ksplit == 1 else t + 2.2 + ksplit * m * n * 8 / 5.5e6
+    return t if ksplit == 1 else t + 3.7 + ksplit * m * n * 1.7e-6
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2596,9 +2597,9 @@ def mx_plan(m: int, n: int, kb: int, big: bool, gated: bool = False) -> Tuple[in
     for mt in (2, 4, 8):
         if 16 * mt > max(32, 2 * m):
             break
-        for ksplit in (1, 2, 4, 8, 16):
-            nt = 4 if gated and ksplit == 1 else 2
-            if (mt, nt) not in _MX_RING or (ksplit > 1 and kb // ksplit < 3):
+        for ksplit in (1, 2, 3, 4, 6, 8, 16):
+            nt = 4 if mt == 8 or (gated and ksplit == 1) else 2
+            if (mt, nt) not in _MX_RING or (gated and mt == 4) or (ksplit > 1 and kb // ksplit < 3):
                 continue
             t = _mx_estimate(m, n, kb, mt, nt, ksplit)
             if t < best:
@@ -2677,12 +2678,13 @@ def mx_gate_up(x, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float,
 
 
 def mx_tile_rows(slots: int, experts: int) -> int:
-    """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices: 16 stream their weights, 32 and 64 share them through
-    the ring, 256 are the large tiles.  us of gate and up and down in tiles of 16, 32, 64 and 256: 128 experts of 2880 x 2880 with 8 rows
-    each 293, 320, 338, -, with 16 456, 337, 349, -, with 32 798, 426, 367, 757; 32 experts with 64 363, 179, 154, 218, with 128 668, 318,
-    223, 230, with 250 -, 627, 419, 335; 8 of 4096 x 14336 with 128 -, 543, 362, 350."""
+    """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices: 16 stream their weights, 32 to 128 share them through
+    the ring, 256 are the large tiles.  us of gate and up and down in tiles of 16, 32, 64, 128 and 256: 128 experts of 2880 x 2880 with 8 rows
+    each 291, 317, 340, -, -, with 16 453, 335, 346, -, -, with 32 791, 421, 367, 461, -, with 47 -, 566, 391, 479, -, with 64 -, 711, 511,
+    491, 786, with 94 -, -, 695, 519, 795, with 125 -, -, 860, 687, 806, with 250 -, -, 1635, 1119, 1128; 32 experts with 128 -, -, 226, 209,
+    223, with 188 -, -, 332, 258, 238, with 500 -, -, -, 583, 499; 64 of 2048 x 1408 with 141 -, -, 185, 188, 173."""
     avg = slots / max(1, experts)
-    return 16 if avg <= 10 else 32 if avg <= 24 else 64 if avg <= 128 else 256
+    return 16 if avg <= 10 else 32 if avg <= 24 else 64 if avg <= 56 else 128 if avg <= 136 else 256
 
 
 def mx_sorted_ok(slots: int, w: quant.MxWeight) -> bool:
@@ -2699,13 +2701,14 @@ def mx_sorted_rows(x, src_row: torch.Tensor) -> quant.MxRows:
 def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], rows: quant.MxRows, nt: int, kb: int, gated: bool) -> int:
     assert tiles.dtype == torch.int32 and tiles.dim() == 2 and tiles.shape[1] == 3 and tiles.is_contiguous()
     assert src is None or (src.dtype == torch.int32 and src.dim() == 1 and src.is_contiguous())
-    assert tile_rows in (16, 32, 64, 256), tile_rows
+    assert tile_rows in (16, 32, 64, 128, 256), tile_rows
     assert tile_rows < 256 or src is None, "tiles of 256 rows: the rows themselves, in order"
     _mx_device(rows.payload.get_device(), tiles, src)
     if tile_rows == 256:
         return MX_BIG
     if tile_rows > 16 and mx_big_ok(rows.payload.shape[0], nt, kb):
-        return _mx_shape(tile_rows // 16, 4 if gated else 2, 1)
+        return _mx_shape(tile_rows // 16, 4 if gated or tile_rows == 128 else 2, 1)
+    assert tile_rows < 128, "tiles of 128 rows: within 32-bit byte offsets"
     return _mx_shape(tile_rows // 16, 4, 4)
 
 
