@@ -326,27 +326,41 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
   const int KB = a.KB, SS = (KB + 3) >> 2, KT = (KB + 1) & ~1, ntiles = (a.N + 15) >> 4;
 
   // ---- this workgroup's tiles: bands of 8 row tiles, in a band every XCD a range of tile columns, column by column (as the 16-bit
-  // product's large tiles: 32 workgroups of an XCD share 12 panels in its L2).  Grouped: units of two row tiles and all columns of an
-  // eighth, dealt to the XCDs in turn
+  // product's large tiles: 32 workgroups of an XCD share 12 panels in its L2).  Grouped: two row tiles at a time, column by column, an
+  // eighth of all outputs to each XCD - of the entries that hold rows, so that the unused ones leave nobody idle
   const int xcd = blockIdx.x & 7, stride = gridDim.x >> 3;
   const int c0 = (int)((long)ntn * xcd >> 3), c1 = (int)((long)ntn * (xcd + 1) >> 3), ncols = c1 - c0;
-  const int gparts = ntn >= 16 ? ntn / 8 : 1, gcols = (ntn + gparts - 1) / gparts;
-  const int units = ((ntm + 1) / 2 * gparts - xcd + 7) / 8;
-  const int chunk_end = grouped ? units * 2 * gcols : ntm * ncols;
-  auto unit_of = [&](int tl) { return xcd + 8 * (tl / (2 * gcols)); };
-  auto row_tile = [&](int tl) { return 2 * (unit_of(tl) / gparts) + (tl & 1); };
-  auto column = [&](int tl) { return unit_of(tl) % gparts * gcols + (tl % (2 * gcols) >> 1); };
+  int lo = 0, hi = ntm;                      // the entries with rows (all of them: unused ones are in front and behind)
+  if (grouped) {
+    lo = ntm, hi = 0;
+    for (int i = threadIdx.x; i < ntm; i += 512)
+      if (a.tiles[3 * i + 2] > 0) lo = min(lo, i), hi = i + 1;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) lo = min(lo, __shfl_xor(lo, d)), hi = max(hi, __shfl_xor(hi, d));
+    int* const red = reinterpret_cast<int*>(smem);
+    if (lane == 0) red[wid] = lo, red[8 + wid] = hi;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo = min(lo, red[i]), hi = max(hi, red[8 + i]);
+    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    __syncthreads();
+  }
+  const int pairs = grouped ? max(hi - lo, 0) / 2 * 2 * ntn : 0;      // outputs of whole pairs of row tiles
+  const long all = grouped ? (long)max(hi - lo, 0) * ntn : 0;
+  const int chunk_end = grouped ? (int)(all * (xcd + 1) >> 3) : ntm * ncols;
+  auto row_tile = [&](int tl) { return tl < pairs ? lo + 2 * (tl / (2 * ntn)) + (tl & 1) : hi - 1; };
+  auto column = [&](int tl) { return tl < pairs ? tl % (2 * ntn) >> 1 : tl - pairs; };
   auto entry = [&](int rt, int i) { return __builtin_amdgcn_readfirstlane(a.tiles[3 * rt + i]); };
   auto used = [&](int tl) {                  // the first entry with rows from tl on
     if (grouped)
       while (tl < chunk_end) {
         const int rt = row_tile(tl);
-        if (rt < ntm && column(tl) < ntn && entry(rt, 2) > 0) break;
+        if (entry(rt, 2) > 0) break;
         tl += stride;
       }
     return tl;
   };
-  int tile = used(blockIdx.x >> 3);
+  int tile = used((grouped ? (int)(all * xcd >> 3) : 0) + (blockIdx.x >> 3));
   if (tile >= chunk_end) return;
   auto decode = [&](int tl, int& m0, int& end, int& tn, int& g) {      // first row, row limit, tile column, matrix
     if (grouped) {
@@ -595,9 +609,8 @@ int mx_big(const MxArgs& a, hipStream_t st) {
   if ((long)a.x_rows * a.ldq >= lim || a.lds % 16 || ((a.N + 15L) / 16) * a.KB * 1024 >= lim) return -8;
   const int ntn = EPI == MX_GLU ? (a.N / 2 + 127) / 128 : (a.N + 255) / 256;
   const int ntm = a.tiles != nullptr ? a.num_tiles : (a.M + 255) / 256;
-  const int gparts = ntn >= 16 ? ntn / 8 : 1;
-  const long per = a.tiles != nullptr ? ((ntm + 1L) / 2 * gparts + 7) / 8 * 2 * ((ntn + gparts - 1) / gparts) : (long)ntm * ((ntn + 7) / 8);
-  if (per >= (1L << 30)) return -7;
+  const long per = a.tiles != nullptr ? ((long)ntm * ntn + 7) / 8 : (long)ntm * ((ntn + 7) / 8);
+  if (per >= (1L << 27)) return -7;
   const int cus = mx_num_cus() / 8;
   const unsigned grid = 8 * (unsigned)(per < cus ? per : cus);
   if (a.tiles != nullptr) mx_big_kernel<T, EPI, true><<<grid, 512, 0, st>>>(a, ntm, ntn);

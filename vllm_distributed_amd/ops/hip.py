@@ -2681,8 +2681,8 @@ def mx_tile_rows(slots: int, experts: int) -> int:
     """Rows of a tile of ``moe_align`` for ``slots`` rows over ``experts`` matrices: 16 stream their weights, 32 to 128 share them through
     the ring, 256 are the large tiles.  us of gate and up and down in tiles of 16, 32, 64, 128 and 256: 128 experts of 2880 x 2880 with 8 rows
     each 291, 317, 340, -, -, with 16 453, 335, 346, -, -, with 32 791, 421, 367, 461, -, with 47 -, 566, 391, 479, -, with 64 -, 711, 511,
-    491, 786, with 94 -, -, 695, 519, 795, with 125 -, -, 860, 687, 806, with 250 -, -, 1635, 1119, 1128; 32 experts with 128 -, -, 226, 209,
-    223, with 188 -, -, 332, 258, 238, with 500 -, -, -, 583, 499; 64 of 2048 x 1408 with 141 -, -, 185, 188, 173."""
+    490, 777, with 94 -, -, 695, 512, 781, with 125 -, -, 860, 681, 797, with 250 -, -, 1635, 1126, 1100; 32 experts with 128 -, -, 226, 212,
+    222, with 188 -, -, 332, 260, 231, with 250 -, -, 424, 323, 286, with 500 -, -, -, 581, 495; 64 of 2048 x 1408 with 141 -, -, 185, 186, 172."""
     avg = slots / max(1, experts)
     return 16 if avg <= 10 else 32 if avg <= 24 else 64 if avg <= 56 else 128 if avg <= 136 else 256
 
