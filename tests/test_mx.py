@@ -375,3 +375,13 @@ def test_two_ranks_and_their_saved_shards(model, saves, tmp_path, monkeypatch):
         return
     again = run(shards, "sharded_state")
     assert [t for t, _ in again] == [t for t, _ in two]
+
+
+@pytest.mark.parametrize("model", ["nemotron-tiny", "stablelm-tiny", "cohere-tiny", "phimoe-tiny", "glm4-moe-tiny", "granite-tiny", "arcee-tiny"])
+def test_families_with_other_norms_and_experts(model):
+    """Layers whose norm is not an RMS norm (it hands over no 8-bit rows), whose experts are routed in another way, or whose feed-forward
+    is not gated run on the same projections."""
+    def check(m):
+        assert any(getattr(x, "mx_qw", None) is not None for x in m.modules())
+    for tokens, logprobs in generate(model=model, quantization="mxfp4", load_format="dummy", check=check, tokens=2):
+        assert len(tokens) == 2 and all(abs(v) < 1e4 for lp in logprobs for v in lp.values())

@@ -107,7 +107,8 @@ WIDE = dict(num_hidden_layers=2, num_key_value_heads=2, head_dim=64)
     # reductions long enough to be split over the grid: the sums go to the norm behind the projection, or to the rotation behind q, k and v
     ("llama-tiny", dict(WIDE, hidden_size=512, num_attention_heads=64, intermediate_size=4096), LINEARS | {"mx_gate_up", "mx_linear_partials", "reduce_add_rms_norm_mx"}),
     ("llama-tiny", dict(WIDE, hidden_size=4096, num_attention_heads=4, intermediate_size=4096), LINEARS | {"mx_gate_up", "mx_linear_partials"}),
-    ("mixtral-tiny", {}, LINEARS | {"mx_experts"}), ("qwen3-moe-tiny", {}, LINEARS | {"mx_experts"}), ("gpt-oss-tiny", {}, {"mx_experts"})])
+    ("mixtral-tiny", {}, LINEARS | {"mx_experts"}), ("qwen3-moe-tiny", {}, LINEARS | {"mx_experts"}), ("gpt-oss-tiny", {}, {"mx_experts"}),
+    ("glm4-moe-tiny", {}, LINEARS | {"mx_experts"}), ("phimoe-tiny", {}, {"mx_linear", "mx_experts"}), ("stablelm-tiny", {}, {"mx_linear", "mx_gate_up"})])
 def test_every_call_of_a_model(model, over, calls, monkeypatch):
     seen = Counter()
     watch(monkeypatch, seen)

@@ -278,9 +278,16 @@ class DeepseekMoE(FusedMoE):
         return ops.moe_topk_grouped(logits, bias, self.top_k, self.n_group if grouped else 1,
                                     self.topk_group if grouped else 1, self.v3, self.v3, renorm, scale)
 
+    def _choose(self, logits: torch.Tensor):
+        if self.n_group <= 64 and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
+            return self._route_hip(logits)
+        return self.route(logits.float())
+
     def _forward_routed(self, x: torch.Tensor) -> torch.Tensor:
         """The routed experts' weighted sum (unreduced).  On the GPU: router GEMM, one routing kernel, slot sort +
         tile table, row gather, two grouped GEMMs with the activation between them, weighted combine."""
+        if self.mx13_qw is not None:
+            return super().forward(x, reduce=False)
         tile_rows = self._expert_tile_rows(x) if x.dim() == 2 else 0
         if not tile_rows or self.num_experts > 512 or self.top_k > 16 or self.n_group > 64:
             return super().forward(x, reduce=False)

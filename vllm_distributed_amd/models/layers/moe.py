@@ -194,12 +194,15 @@ class FusedMoE(nn.Module):
         self.mx13_qw, self.mx13_ws = torch.stack([w.qw for w in w13]), torch.stack([w.ws for w in w13])
         self.mx2_qw, self.mx2_ws = torch.stack([w.qw for w in w2]), torch.stack([w.ws for w in w2])
 
+    def _choose(self, logits: torch.Tensor):
+        """``route`` in one kernel where there is one for it."""
+        if not self.custom_routing and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
+            return ops.moe_topk(logits, self.top_k, self.renormalize)
+        return self.route(logits.float())
+
     def _experts_mx(self, x: torch.Tensor, logits: torch.Tensor, **extra) -> torch.Tensor:
         """The experts' products in microscaled floating point (``ops.mx_experts``), behind the router's choice."""
-        if not self.custom_routing and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
-            topw, topi = ops.moe_topk(logits, self.top_k, self.renormalize)
-        else:
-            topw, topi = self.route(logits.float())
+        topw, topi = self._choose(logits)
         weights = (ops.MxWeight(self.mx13_qw, self.mx13_ws, self.mx13_qw.shape[1] * 16),
                    ops.MxWeight(self.mx2_qw, self.mx2_ws, self.hidden))
         return ops.mx_experts(x, topw.float().contiguous(), topi.to(torch.int32).contiguous(), *weights, expert_start=self.expert_start,

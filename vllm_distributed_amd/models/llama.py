@@ -270,7 +270,8 @@ class LlamaDecoderLayer(nn.Module):
         """``hidden`` None (in or out): the producing GEMM has already added its product into
         ``residual`` (large unsharded batches), so the norm that follows is a plain one."""
         # projections with microscaled weights take their input as the 8-bit rows that the norm in front of them leaves
-        rows8 = {"rows8": True} if self._attn_partials and self.self_attn.qkv_proj.takes_rows8 else {}
+        rows8 = ({"rows8": True} if self._attn_partials and self.self_attn.qkv_proj.takes_rows8 and type(self.input_layernorm) is RMSNorm
+                 else {})
         if residual is None:
             residual = hidden
             hidden = self.input_layernorm(hidden, **rows8)
@@ -282,7 +283,8 @@ class LlamaDecoderLayer(nn.Module):
             hidden = self.self_attn(positions, hidden, residual=residual, partials=True)
         else:
             hidden = self.self_attn(positions, hidden, residual=residual)
-        rows8 = {"rows8": True} if self._mlp_partials and self.mlp.gate_up_proj.takes_rows8 else {}
+        rows8 = ({"rows8": True} if self._mlp_partials and self.mlp.gate_up_proj.takes_rows8
+                 and type(self.post_attention_layernorm) is RMSNorm else {})
         if hidden is None:
             hidden = self.post_attention_layernorm(residual, **rows8)
         else:
