@@ -232,7 +232,7 @@ __global__ __launch_bounds__(ALIGN_THREADS) void moe_align_kernel(
       for (int i = 0; i < 8; ++i) e[i] = s0 + i * ALIGN_THREADS < last ? topi[s0 + i * ALIGN_THREADS] : -1;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (e[i] >= 0) f(s0 + i * ALIGN_THREADS, e[i]);
+        if ((unsigned)e[i] < (unsigned)E) f(s0 + i * ALIGN_THREADS, e[i]);
     }
   };
   each(0, lo, [&](int, int e) { atomicAdd(&cursor[e], 1); });

@@ -918,7 +918,7 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(T* __restrict__ out, co
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int j = 0; j < k; ++j) {
     const int e = topi[t * k + j];
-    if (local >= 0 && (e < first || e >= first + local)) continue;
+    if (e < first || e >= first + local) continue;
     const int row = min(max(at[t * k + j], 0), rows - 1);
     const float w = topw[t * k + j];
     const f32x4 v = *reinterpret_cast<const f32x4*>(y + (long)row * H + c);
@@ -1069,8 +1069,8 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
   return -2;
 }
 
-// y [tokens k][H] 32-bit rows (H % 4 == 0), topw and topi [tokens][k], at [tokens k]: the row of each slot -> out [tokens][H].  local >= 0:
-// only slots of experts first .. first + local - 1
+// y [tokens k][H] 32-bit rows (H % 4 == 0), topw and topi [tokens][k], at [tokens k]: the row of each slot -> out [tokens][H], of the slots
+// of experts first .. first + local - 1
 VDAMD_API int vdamd_mx_combine(void* out, const float* y, const float* topw, const int* topi, const int* at, int tokens, int k, int H,
                                int first, int local, int dtype, void* stream) {
   if (tokens <= 0) return 0;

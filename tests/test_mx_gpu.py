@@ -372,6 +372,23 @@ def test_experts(t, e, k, h, inter, limit):
     assert off.norm() <= 2.0 ** -6 * want.norm()
 
 
+@pytest.mark.parametrize("t", [3, 40, 200, 600])
+def test_experts_nobody_has(t):
+    """Slots of numbers that are no expert's add nothing, at each kind of tile; no rows are none."""
+    from vllm_distributed_amd import ops
+    e, k, h, inter = 4, 3, 96, 160
+    x = (rows(t, h, spread=0.3).float() / h ** 0.5).to(torch.bfloat16)
+    w13, v13 = make_experts(e, 2 * inter, h, halves=2)
+    w2, v2 = make_experts(e, h, inter)
+    topi = torch.stack([torch.randperm(e)[:k] for _ in range(t)]).int()
+    topi[::2, 1], topi[1::3, 2], topi[0] = -1, e + 5, -7
+    topw = torch.rand(t, k)
+    y = ops.mx_experts(x.cuda(), topw.cuda(), topi.cuda(), w13, w2)
+    want, bound = expert_block(oracle.blocks(x, 8)[2], topw, topi, v13, v2, None, None, 0.0)
+    assert ((y.cpu().double() - want).abs() <= bound).all() and not y[0].any()
+    assert ops.mx_experts(x[:0].cuda(), topw[:0].cuda(), topi[:0].cuda(), w13, w2).shape == (0, h)
+
+
 @pytest.mark.parametrize("t", [5, 33, 700])
 def test_experts_of_two_ranks_add_up(t):
     """Expert parallel: each rank adds its experts' part; in one row's 32-bit sum the parts are those of the whole block."""

@@ -599,7 +599,8 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
     """A sparse block behind its router: ``sum_j topw[t, j] down_e(gated_e(x[t]))``, ``e = topi[t, j]``, for experts whose matrices are
     4-bit microscaled (``weight13`` ``[E, gate ; up]`` packed with ``halves=2``, ``weight2 [E, H]``) with biases ``[E, rows]``.  ``x [T, H]``
     16-bit rows or an ``MxRows``, ``topw [T, k]`` fp32, ``topi [T, k]`` int32.  ``expert_start`` / ``local_experts`` (expert parallel): the
-    matrices are those of experts ``expert_start ..``, other slots add nothing; ``num_experts``: the router's outputs then."""
+    matrices are those of experts ``expert_start ..``; ``num_experts``: the router's outputs then.  Slots of other numbers (-1: nobody) add
+    nothing."""
     e_local = weight13.qw.shape[0]
     total = num_experts or (e_local if local_experts < 0 else expert_start + local_experts)
     t, k = topi.shape
@@ -624,7 +625,7 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
             rows = x if isinstance(x, MxRows) else _hip.mx_quantize(x, 8)
         a = _hip.mx_grouped_gate_up(rows, weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
         y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2, wide=True)      # (summed in 32 bits, rounded once)
-        return _hip.mx_combine(y, topw, topi, inv, dtype, expert_start, local_experts)
+        return _hip.mx_combine(y, topw, topi, inv, dtype, expert_start if local_experts >= 0 else 0, e_local)
     return torch_ref.mx_experts(_mx_operand(x, weight13), topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)
 
 

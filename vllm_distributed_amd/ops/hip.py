@@ -2726,9 +2726,9 @@ def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor
     return out
 
 
-def mx_combine(y: torch.Tensor, topw: torch.Tensor, topi: torch.Tensor, inv: torch.Tensor, dtype: torch.dtype, expert_start: int = 0,
-               local_experts: int = -1) -> torch.Tensor:
-    """``moe_combine`` of 32-bit rows: rounded once."""
+def mx_combine(y: torch.Tensor, topw: torch.Tensor, topi: torch.Tensor, inv: torch.Tensor, dtype: torch.dtype, expert_start: int,
+               local_experts: int) -> torch.Tensor:
+    """``moe_combine`` of 32-bit rows, rounded once; slots of other experts than the local ones add nothing."""
     t, k = topi.shape
     h = y.shape[1]
     assert y.dtype == torch.float32 and y.is_contiguous() and h % 4 == 0 and y.shape[0] == t * k and inv.numel() == t * k
