@@ -261,6 +261,68 @@ def test_every_shape_of_the_ring(m, n, k, mt, nt, ksplit, monkeypatch):
         check_rows(ops.mx_gate_up(xr, w), v, slack)
 
 
+@pytest.mark.parametrize("m", [17, 40, 130])
+def test_operands_past_32_bit_offsets_stream(m, monkeypatch):
+    """What runs for operands of 4 GiB and more, at small ones."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    monkeypatch.setattr(hip, "mx_big_ok", lambda *a: False)
+    monkeypatch.setattr(hip, "mx_sorted_ok", lambda *a: False)
+    x = (rows(m, 1056).float() / 32).to(torch.bfloat16)
+    w, wv = make(264, 1056)
+    check_product(ops.mx_linear(x.cuda(), w), oracle.blocks(x, 8)[2], wv, torch.bfloat16)
+    w, wv = make(512, 1056, halves=2, spread=1)
+    v, slack = gated_slack(oracle.blocks(x, 8)[2], wv, None, 0.0)
+    check_rows(ops.mx_gate_up(x.cuda(), w), v, slack)
+    w13, v13 = make_experts(2, 256, 1056, halves=2)
+    w2, v2 = make_experts(2, 96, 128)
+    topi = torch.stack([torch.randperm(2) for _ in range(m)]).int()
+    topw = torch.rand(m, 2)
+    y = ops.mx_experts(x.cuda(), topw.cuda(), topi.cuda(), w13, w2)
+    want, bound = expert_block(oracle.blocks(x, 8)[2], topw, topi, v13, v2, None, None, 0.0)
+    assert ((y.cpu().double() - want).abs() <= bound).all()
+
+
+def test_rows_of_4_gib():
+    """530 000 rows of 8192: payload past 32-bit offsets.  Rows from both ends and the middle."""
+    from vllm_distributed_amd import ops
+    m, k = 530_000, 8192
+    some = torch.tensor([0, 1, 262_143, 262_144, 524_287, 524_288, m - 1])
+    seven = rows(7, k)
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[some.cuda()] = seven.cuda()
+    w, wv = make(24, k)
+    r = ops.mx_quantize(x)
+    del x
+    y = ops.mx_linear(r, w)
+    check_product(y[some.cuda()], oracle.blocks(seven, 8)[2], wv, torch.bfloat16)
+    y[some.cuda()] = 0
+    assert not y.any()
+    back = ops.mx_dequantize(ops.MxRows(r.payload[-2:], r.scales[-2:], k, 8, r.dtype), torch.float32)
+    assert torch.equal(back[1].cpu().double(), oracle.blocks(seven, 8)[2][6])
+
+
+@pytest.mark.parametrize("m", [2, 40])
+def test_weight_of_4_gib(m):
+    """1 056 000 columns of 8192: the weight's tiles past 32-bit offsets.  Columns from both ends and beside the border."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import quant
+    n, k = 1_056_000, 8192
+    q, s, wv = oracle.random_weight(48, k, torch.Generator().manual_seed(m), 1)
+    part = quant.pack_mx(q.cuda(), s.cuda())
+    w = ops.MxWeight(torch.zeros(n // 16, k // 128, 64, 4, dtype=torch.int32, device="cuda"),
+                     torch.zeros(n // 16, k // 512, 64, 4, dtype=torch.uint8, device="cuda"), n)
+    at = [0, 65_536, n // 16 - 1]
+    for i, t in enumerate(at):
+        w.qw[t], w.ws[t] = part.qw[i], part.ws[i]
+    x = rows(m, k, spread=0.3)
+    y = ops.mx_linear(x.cuda(), w)
+    for i, t in enumerate(at):
+        check_product(y[:, 16 * t:16 * t + 16], oracle.blocks(x, 8)[2], wv[16 * i:16 * i + 16], torch.bfloat16)
+        y[:, 16 * t:16 * t + 16] = 0
+    assert not y.any()
+
+
 @pytest.mark.parametrize("m,n,k", [(40, 512, 4096), (64, 2880, 4096)])
 def test_partials_and_the_norm_behind_them(m, n, k):
     from vllm_distributed_amd import ops
@@ -383,9 +445,10 @@ def test_experts_nobody_has(t):
     topi = torch.stack([torch.randperm(e)[:k] for _ in range(t)]).int()
     topi[::2, 1], topi[1::3, 2], topi[0] = -1, e + 5, -7
     topw = torch.rand(t, k)
-    y = ops.mx_experts(x.cuda(), topw.cuda(), topi.cuda(), w13, w2)
     want, bound = expert_block(oracle.blocks(x, 8)[2], topw, topi, v13, v2, None, None, 0.0)
-    assert ((y.cpu().double() - want).abs() <= bound).all() and not y[0].any()
+    for rows_ in (x.cuda(), ops.mx_quantize(x.cuda())):
+        y = ops.mx_experts(rows_, topw.cuda(), topi.cuda(), w13, w2)
+        assert ((y.cpu().double() - want).abs() <= bound).all() and not y[0].any()
     assert ops.mx_experts(x[:0].cuda(), topw[:0].cuda(), topi[:0].cuda(), w13, w2).shape == (0, h)
 
 

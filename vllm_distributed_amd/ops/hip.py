@@ -2694,8 +2694,8 @@ def mx_sorted_ok(slots: int, w: quant.MxWeight) -> bool:
 
 
 def mx_sorted_rows(x, src_row: torch.Tensor) -> quant.MxRows:
-    """``x[src_row]`` in 8 bits, ``x`` 16-bit rows or ``MxRows``."""
-    return x.take(src_row) if isinstance(x, quant.MxRows) else mx_quantize(x, 8, src_row=src_row)
+    """``x[src_row]`` in 8 bits, ``x`` 16-bit rows or ``MxRows`` (numbers of no row, which no tile has: of any)."""
+    return x.take(src_row.clamp(0, x.shape[0] - 1)) if isinstance(x, quant.MxRows) else mx_quantize(x, 8, src_row=src_row)
 
 
 def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], rows: quant.MxRows, nt: int, kb: int, gated: bool) -> int:
