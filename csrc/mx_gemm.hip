@@ -46,14 +46,18 @@ template <typename P> __device__ __forceinline__ mx_i32x8 mx_fragment(const P* l
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-__device__ __forceinline__ float mx_glu(float g, float u, float limit, float alpha) {
-  if (limit > 0.f) {
-    g = g > limit ? limit : g;                      // (a NaN stays one)
-    u = u > limit ? limit : (u < -limit ? -limit : u);
-    return (u + 1.f) * g * fast_sigmoid(alpha * g);
+// Both forms as (u' + plus) g' sigmoid(alpha g') with u' = u limited to +-top, g' = g to top: SiLU has no limit.  (A branch for each value
+// keeps the next one's exponential from starting under it: 22528 x 5888 x 2944 in 256-row tiles 395 us with limits, 365 without; so 349, 340.)
+struct MxGlu {
+  float top, plus, alpha;
+  __device__ __forceinline__ MxGlu(float limit, float a) : top(limit > 0.f ? limit : __uint_as_float(0x7f800000u)),
+                                                           plus(limit > 0.f ? 1.f : 0.f), alpha(limit > 0.f ? a : 1.f) {}
+  __device__ __forceinline__ float operator()(float g, float u) const {
+    g = g > top ? top : g;                          // (a NaN stays one)
+    u = u > top ? top : (u < -top ? -top : u);
+    return (u + plus) * g * fast_sigmoid(alpha * g);
   }
-  return g * fast_sigmoid(g) * u;
-}
+};
 
 // A row's block of 32 gated values is with four lanes (r, q), 4 columns from 4 q of both its 16-column halves: elements and scale.  All
 // 64 lanes run; ok: the row is stored
@@ -224,6 +228,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(const MxArgs a) {
   };
   if constexpr (EPI == MX_GLU) {
     const int cols = a.N >> 1, n = 32 * blockIdx.x + 4 * q;
+    const MxGlu glu(a.limit, a.alpha);
     for (int i = wid; i < MT; i += WAVES) {
       const int m = 16 * i + r;
       float v[2][4];
@@ -233,7 +238,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(const MxArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int c = n + 16 * h + e;
-          v[h][e] = mx_glu(g[e] + (bias ? (float)bias[c] : 0.f), u[e] + (bias ? (float)bias[cols + c] : 0.f), a.limit, a.alpha);
+          v[h][e] = glu(g[e] + (bias ? (float)bias[c] : 0.f), u[e] + (bias ? (float)bias[cols + c] : 0.f));
         }
       }
       const long row = row0 + min(m, rows - 1);
@@ -539,6 +544,7 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
     float b0[2][4], b1[2][4];
     mx_bias<T>(b0, a.bias, (long)cg * a.N, n0, a.N, eq);
     mx_bias<T>(b1, a.bias, (long)cg * a.N, n1, a.N, eq);
+    [[maybe_unused]] const MxGlu glu(a.limit, a.alpha);
     auto put = [&](const f32x4 (&a0)[4][2], const f32x4 (&a1)[4][2], int mq) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -548,7 +554,7 @@ __global__ __launch_bounds__(512) void mx_big_kernel(const MxArgs a, int ntm, in
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][e] = mx_glu(a0[i][j][e] + b0[j][e], a1[i][j][e] + b1[j][e], a.limit, a.alpha);
+            for (int e = 0; e < 4; ++e) v[j][e] = glu(a0[i][j][e] + b0[j][e], a1[i][j][e] + b1[j][e]);
           mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n0, a.os + (long)m * a.ldos + (n0 >> 5), v, eln, m < cend);
         } else if constexpr (EPI == MX_SLAB) {
 #pragma unroll
@@ -823,6 +829,7 @@ __global__ __launch_bounds__(256 * WM) void mx_ring_kernel(const MxArgs a) {
     float b0[2][4], b1[2][4];
     mx_bias<T>(b0, a.bias, (long)group * a.N, n0, a.N, q);
     mx_bias<T>(b1, a.bias, (long)group * a.N, n1, a.N, q);
+    const MxGlu glu(a.limit, a.alpha);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int m = row0 + 16 * (MT * wm + i) + r;
@@ -830,7 +837,7 @@ __global__ __launch_bounds__(256 * WM) void mx_ring_kernel(const MxArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = mx_glu(acc[j][i][e] + b0[j][e], acc[2 + j][i][e] + b1[j][e], a.limit, a.alpha);
+        for (int e = 0; e < 4; ++e) v[j][e] = glu(acc[j][i][e] + b0[j][e], acc[2 + j][i][e] + b1[j][e]);
       mx_store_block((uint8_t*)a.out + (long)m * a.ldo + n0, a.os + (long)m * a.ldos + (n0 >> 5), v, lane, m < end);
     }
   } else {
@@ -900,8 +907,9 @@ __global__ __launch_bounds__(256) void mx_reduce_glu_kernel(uint8_t* __restrict_
 #pragma unroll
     for (int e = 0; e < 8; ++e) { g[e] += a[e]; u[e] += b[e]; }
   }
+  const MxGlu glu(limit, alpha);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = mx_glu(g[e], u[e], limit, alpha);
+  for (int e = 0; e < 8; ++e) v[e] = glu(g[e], u[e]);
   mx_store8(out + m * ldo + c, os + m * ldos + (c >> 5), v);
 }
 
