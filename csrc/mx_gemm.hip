@@ -619,9 +619,10 @@ int mx_big(const MxArgs& a, hipStream_t st) {
   if (per >= (1L << 27)) return -7;
   const int cus = mx_num_cus() / 8;
   const unsigned grid = 8 * (unsigned)(per < cus ? per : cus);
-  if (a.tiles != nullptr) mx_big_kernel<T, EPI, true><<<grid, 512, 0, st>>>(a, ntm, ntn);
-  else if constexpr (EPI != MX_SLAB) mx_big_kernel<T, EPI, false><<<grid, 512, 0, st>>>(a, ntm, ntn);
-  else return -6;
+  if constexpr (EPI != MX_OUT)
+    if (a.tiles != nullptr) mx_big_kernel<T, EPI, true><<<grid, 512, 0, st>>>(a, ntm, ntn);
+  if constexpr (EPI != MX_SLAB)
+    if (a.tiles == nullptr) mx_big_kernel<T, EPI, false><<<grid, 512, 0, st>>>(a, ntm, ntn);
   HIP_LAUNCH_CHECK();
   return 0;
 }
@@ -966,11 +967,10 @@ int mx_stream(const MxArgs& a, int mt, int nt, int waves, hipStream_t st) {
     else if (mt == 2) GO(2, 4, 4, false, 2);
     else if (mt == 4) GO(4, 4, 4, false, 2);
     else return -6;
-  } else if (nt == 4 && waves == 8 && mt == 1) {
-    if constexpr (EPI != MX_SLAB) {
-      if (quant) GO(1, 4, 8, true, 3);
-      else GO(1, 4, 8, false, 3);
-    }
+  } else if constexpr (EPI == MX_GLU) {
+    if (nt != 4 || waves != 8 || mt != 1) return -6;
+    if (quant) GO(1, 4, 8, true, 3);
+    else GO(1, 4, 8, false, 3);
   } else if constexpr (EPI == MX_OUT) {
     if (mt != 1 || waves != 8 || (nt != 1 && nt != 2)) return -6;
     if (nt == 1 && quant) GO(1, 1, 8, true, 6);
@@ -1011,7 +1011,7 @@ int mx_ring(const MxArgs& a, int mt, int nt, hipStream_t st) {
 template <typename T>
 int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t st) {
   if (mt == 16) {
-    if (a.ksplit != 1 || a.src != nullptr || a.x16 != nullptr) return -1;
+    if (a.ksplit != 1 || a.src != nullptr || a.x16 != nullptr || (epi == MX_SLAB && a.tiles == nullptr)) return -1;
     return epi == MX_GLU ? mx_big<T, MX_GLU>(a, st) : epi == MX_OUT ? mx_big<T, MX_OUT>(a, st) : mx_big<T, MX_SLAB>(a, st);
   }
   const bool ring = waves == 1;
@@ -1047,7 +1047,7 @@ int mx_dispatch(const MxArgs& a, int epi, int mt, int nt, int waves, hipStream_t
 // epi 0: out [M][N] of the model type, rows ldo elements apart (ksplit > 1: through partial [ksplit][M][N]); 1: partial alone (a bias with
 // ksplit 1 only);
 // 2: N = [gate ; up], N % 256 == 0: out [M][N / 2] elements, os their scales (ksplit > 1: through partial); limit 0: SiLU.
-// tiles [num_tiles][3] (matrix, first row, rows; ksplit 1) or null; src [M] or null: the row of x behind each row.
+// tiles [num_tiles][3] (matrix, first row, rows; ksplit 1, epi 1 or 2) or null; src [M] or null: the row of x behind each row.
 // shape: 16-row tiles a workgroup takes (of `tiles` at most 16 times as many rows each) + 256 times its 16-column tiles + 65536 times its
 // waves for the streaming kernel (mx_stream);  row tiles 2 or 4 + 256 times 2 (4 where epi is 2 and ksplit 1), or 8 + 256 times 4, + 65536:
 // the ring of LDS;
@@ -1068,6 +1068,7 @@ VDAMD_API int vdamd_mx_gemm(void* out, long ldo, void* os, long ldos, float* par
   if (epi == MX_OUT && (ldo % 8 || ldo < N || (uintptr_t)out % 16 || (ksplit > 1 && partial == nullptr))) return -1;
   if (epi == MX_SLAB && partial == nullptr) return -1;
   if (ksplit > 1 && (tiles != nullptr || (epi == MX_SLAB && bias != nullptr))) return -1;
+  if (tiles != nullptr && epi == MX_OUT) return -1;
   if (epi < 0 || epi > 2) return -1;
   const MxArgs a = {(const uint8_t*)xq, ldq, (const uint8_t*)xs, lds, (const uint8_t*)qw, (const uint8_t*)ws, out, ldo, (uint8_t*)os, ldos,
                     partial, bias, M, N, KB, ksplit, limit, alpha, tiles, num_tiles, groups, src, x_rows, x16, ldx, K};

@@ -624,7 +624,7 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
         else:
             rows = x if isinstance(x, MxRows) else _hip.mx_quantize(x, 8)
         a = _hip.mx_grouped_gate_up(rows, weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
-        y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2, wide=True)      # (summed in 32 bits, rounded once)
+        y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2)      # (summed in 32 bits, rounded once)
         return _hip.mx_combine(y, topw, topi, inv, dtype, expert_start if local_experts >= 0 else 0, e_local)
     return torch_ref.mx_experts(_mx_operand(x, weight13), topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)
 

@@ -2712,17 +2712,15 @@ def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], 
     return _mx_shape(tile_rows // 16, 4, 4)
 
 
-def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int, bias: Optional[torch.Tensor] = None,
-                      src_row: Optional[torch.Tensor] = None, wide: bool = False) -> torch.Tensor:
-    """Product of rows sorted by matrix (``moe_align``) with ``w``'s matrices; ``src_row``: the rows are ``rows[src_row]``.  Rows of no
-    tile stay unwritten.  ``wide``: as the 32-bit sums."""
+def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor, tile_rows: int,
+                      bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Product of rows sorted by matrix (``moe_align``) with ``w``'s matrices, as 32-bit rows (which ``mx_combine`` sums).  Rows of no tile
+    stay unwritten."""
     groups, nt, kb = _mx_check(rows, w, bias, True)
-    mt = _mx_tiles(tiles, tile_rows, src_row, rows, nt, kb, False)
-    out = torch.empty((rows.shape[0] if src_row is None else src_row.numel(), w.rows), dtype=torch.float32 if wide else rows.dtype,
-                      device=rows.device)
+    mt = _mx_tiles(tiles, tile_rows, None, rows, nt, kb, False)
+    out = torch.empty((rows.shape[0], w.rows), dtype=torch.float32, device=rows.device)
     if out.shape[0]:
-        _mx_gemm(int(wide), rows, w, groups, kb, bias, None if wide else out, w.rows, None, 0, out if wide else None, (mt, 1), tiles=tiles,
-                 src=src_row)
+        _mx_gemm(1, rows, w, groups, kb, bias, None, w.rows, None, 0, out, (mt, 1), tiles=tiles)
     return out
 
 
