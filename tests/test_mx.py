@@ -123,6 +123,7 @@ def test_refusals():
             (lambda: ops.mx_gate_up(x, w), ValueError),
             (lambda: ops.mx_experts(x, topw, topi, e3, e3, local_experts=1), ValueError),
             (lambda: ops.mx_experts(x, topw, topi, e3, e3, local_experts=2, num_experts=4), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, e3, e3, num_experts=2), ValueError),
             (lambda: ops.mx_experts(x[:3], topw, topi, e3, e3), ValueError),
             (lambda: ops.mx_experts(x, topw, topi[:, :0], e3, e3), ValueError),
             (lambda: quant.pack_mx(q[:60], s[:60]), ValueError), (lambda: quant.pack_mx(q[:24], s[:24], halves=2), ValueError),

@@ -434,6 +434,29 @@ def test_experts(t, e, k, h, inter, limit):
     assert off.norm() <= 2.0 ** -6 * want.norm()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t", [1, 7, 16, 17, 300])
+@pytest.mark.parametrize("e,k", [(8, 2), (64, 6), (3, 3)])
+def test_experts_behind_their_router(t, e, k, dtype):
+    """The same bits as the choice and the experts in calls of their own, whole and in two ranks' halves."""
+    from vllm_distributed_amd import ops
+    h, inter = 160, 128
+    x = (rows(t, h, spread=0.3).float() / h ** 0.5).to(dtype).cuda()
+    w13, _ = make_experts(e, 2 * inter, h, halves=2)
+    w2, _ = make_experts(e, h, inter)
+    b2 = torch.randn(e, h).to(dtype).cuda()
+    for logits in (torch.randn(t, e).cuda(), torch.randn(t, e).to(dtype).cuda()):
+        topw, topi = ops.moe_topk(logits, k, True)
+        want = ops.mx_experts(x, topw, topi, w13, w2, None, b2, limit=7.0)
+        assert torch.equal(ops.mx_experts_routed(logits, x, k, True, w13, w2, None, b2, limit=7.0), want)
+        part = lambda w, lo, n: ops.MxWeight(w.qw[lo:lo + n].contiguous(), w.ws[lo:lo + n].contiguous(), w.rows)
+        for lo, n in ((0, e // 2), (e // 2, e - e // 2)):
+            args = part(w13, lo, n), part(w2, lo, n), None, b2[lo:lo + n].contiguous(), lo, n
+            assert torch.equal(ops.mx_experts_routed(logits, x, k, True, *args), ops.mx_experts(x, topw, topi, *args, e))
+    with pytest.raises(ValueError):
+        ops.mx_experts_routed(torch.randn(t, e + 1).cuda(), x, k, True, w13, w2)
+
+
 @pytest.mark.parametrize("t", [3, 40, 200, 600])
 def test_experts_nobody_has(t):
     """Slots of numbers that are no expert's add nothing, at each kind of tile; no rows are none."""

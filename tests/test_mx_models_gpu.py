@@ -41,7 +41,7 @@ def numbers(x):
 
 def watch(monkeypatch, seen):
     """Every microscaled call that a model makes, against 64 bits over the operands it got, with the bounds of the operators' own tests."""
-    real = {n: getattr(ops, n) for n in ("mx_linear", "mx_linear_partials", "mx_gate_up", "mx_experts", "rms_norm_mx",
+    real = {n: getattr(ops, n) for n in ("mx_linear", "mx_linear_partials", "mx_gate_up", "mx_experts", "mx_experts_routed", "rms_norm_mx",
                                          "fused_add_rms_norm_mx", "reduce_add_rms_norm_mx")}
 
     def product(x, w, bias=None):
@@ -92,7 +92,19 @@ def watch(monkeypatch, seen):
             assert (off <= bound).all(), f"worst {(off / bound).max():.3g} of the bound"
             seen["mx_experts"] += 1
         return y
-    for name, f in (("mx_linear", product), ("mx_linear_partials", partials), ("mx_gate_up", gate_up), ("mx_experts", experts),
+
+    def routed(logits, x, k, renormalize, w13, w2, bias13=None, bias2=None, limit=0.0, **kw):
+        y = real["mx_experts_routed"](logits, x, k, renormalize, w13, w2, bias13=bias13, bias2=bias2, limit=limit, **kw)
+        if x.shape[0] <= 16:
+            topw, topi = ops.moe_topk(logits.sum(0) if logits.dim() == 3 else logits, k, renormalize)
+            want, bound = expert_block(numbers(x), topw.cpu(), topi.cpu(), dense(w13)[..., :x.shape[1]], dense(w2)[..., :w13.rows // 2], bias13,
+                                       bias2, limit)
+            # (sums of the router's parts in another order: the weights are off by a few 2^-24 times the logits' size)
+            off = (y.cpu().double() - want).abs()
+            assert (off <= bound + 2.0 ** -18 * want.abs()).all(), f"worst {(off / bound).max():.3g} of the bound"
+            seen["mx_experts_routed"] += 1
+        return y
+    for name, f in (("mx_linear", product), ("mx_linear_partials", partials), ("mx_gate_up", gate_up), ("mx_experts", experts), ("mx_experts_routed", routed),
                     ("rms_norm_mx", norm("rms_norm_mx")), ("fused_add_rms_norm_mx", norm("fused_add_rms_norm_mx")),
                     ("reduce_add_rms_norm_mx", norm("reduce_add_rms_norm_mx", True))):
         monkeypatch.setattr(ops, name, f)
@@ -107,7 +119,8 @@ WIDE = dict(num_hidden_layers=2, num_key_value_heads=2, head_dim=64)
     # reductions long enough to be split over the grid: the sums go to the norm behind the projection, or to the rotation behind q, k and v
     ("llama-tiny", dict(WIDE, hidden_size=512, num_attention_heads=64, intermediate_size=4096), LINEARS | {"mx_gate_up", "mx_linear_partials", "reduce_add_rms_norm_mx"}),
     ("llama-tiny", dict(WIDE, hidden_size=4096, num_attention_heads=4, intermediate_size=4096), LINEARS | {"mx_gate_up", "mx_linear_partials"}),
-    ("mixtral-tiny", {}, LINEARS | {"mx_experts"}), ("qwen3-moe-tiny", {}, LINEARS | {"mx_experts"}), ("gpt-oss-tiny", {}, {"mx_experts"}),
+    ("mixtral-tiny", {}, LINEARS | {"mx_experts", "mx_experts_routed"}), ("qwen3-moe-tiny", {}, LINEARS | {"mx_experts", "mx_experts_routed"}),
+    ("gpt-oss-tiny", {}, {"mx_experts", "mx_experts_routed"}),
     ("glm4-moe-tiny", {}, LINEARS | {"mx_experts"}), ("phimoe-tiny", {}, {"mx_linear", "mx_experts"}), ("stablelm-tiny", {}, {"mx_linear", "mx_gate_up"})])
 def test_every_call_of_a_model(model, over, calls, monkeypatch):
     seen = Counter()

@@ -192,10 +192,10 @@ class GptOssMoE(FusedMoE):
         return ops.moe_combine(y, topw, topi, inv, self.expert_start, local, bias=self.b2)
 
     def forward(self, x: torch.Tensor, reduce: bool = True, staged: bool = False, deferred: bool = False):
-        logits = self.gate(x)
         if self.mx13_qw is not None:
-            out = self._experts_mx(x, logits, bias13=self.b13, bias2=self.b2, limit=self.limit, alpha=self.ALPHA)
+            out = self._experts_mx(x, bias13=self.b13, bias2=self.b2, limit=self.limit, alpha=self.ALPHA)
             return tensor_model_parallel_all_reduce(out) if reduce and self.tp > 1 else out
+        logits = self.gate(x)
         tile_rows = self._expert_tile_rows(x)
         if tile_rows and x.dim() == 2 and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
             out = self._forward_fused_routing(x, logits, tile_rows)

@@ -196,17 +196,22 @@ class FusedMoE(nn.Module):
 
     def _choose(self, logits: torch.Tensor):
         """``route`` in one kernel where there is one for it."""
-        if not self.custom_routing and ops.moe_route_fused_ok(logits, self.num_experts, self.top_k):
-            return ops.moe_topk(logits, self.top_k, self.renormalize)
         return self.route(logits.float())
 
-    def _experts_mx(self, x: torch.Tensor, logits: torch.Tensor, **extra) -> torch.Tensor:
-        """The experts' products in microscaled floating point (``ops.mx_experts``), behind the router's choice."""
-        topw, topi = self._choose(logits)
+    def _experts_mx(self, x: torch.Tensor, **extra) -> torch.Tensor:
+        """The router's choice and the experts' products in microscaled floating point (``ops.mx_experts``)."""
+        logits = None
+        if not self.custom_routing and self.gate.bias is None and getattr(self.gate, "lora", None) is None and x.dim() == 2:
+            logits = ops.router_logit_partials(x, self.gate.weight)     # (their sum is left to the routing kernel)
+        if logits is None:
+            logits = self.router_logits(x)
         weights = (ops.MxWeight(self.mx13_qw, self.mx13_ws, self.mx13_qw.shape[1] * 16),
                    ops.MxWeight(self.mx2_qw, self.mx2_ws, self.hidden))
-        return ops.mx_experts(x, topw.float().contiguous(), topi.to(torch.int32).contiguous(), *weights, expert_start=self.expert_start,
-                              local_experts=self.local_experts if self.expert_parallel else -1, num_experts=self.num_experts, **extra)
+        extra.update(expert_start=self.expert_start, local_experts=self.local_experts if self.expert_parallel else -1)
+        if not self.custom_routing and (logits.dim() == 3 or ops.moe_route_fused_ok(logits, self.num_experts, self.top_k)):
+            return ops.mx_experts_routed(logits, x, self.top_k, self.renormalize, *weights, **extra)
+        topw, topi = self._choose(logits)
+        return ops.mx_experts(x, topw.float().contiguous(), topi.to(torch.int32).contiguous(), *weights, num_experts=self.num_experts, **extra)
 
     def _finalize_nvfp4(self) -> None:
         from ...ops import quant
@@ -348,7 +353,7 @@ class FusedMoE(nn.Module):
         # `deferred`: the caller feeds the result to an add + RMSNorm and accepts ``ExpertRows``
         # `staged` (write the partial sums where the next direct all-reduce reads) is a hint only
         if self.mx13_qw is not None:
-            out = self._experts_mx(x, self.router_logits(x))
+            out = self._experts_mx(x)
             return tensor_model_parallel_all_reduce(out) if reduce and self.tp > 1 else out
         tile_rows = self._expert_tile_rows(x)
         logits = None

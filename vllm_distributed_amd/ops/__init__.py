@@ -612,6 +612,8 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
     dtype = x.dtype
     if local_experts >= 0 and not num_experts:
         raise ValueError("the number of the router's outputs is wanted beside local_experts")
+    if local_experts < 0 and num_experts not in (0, e_local):
+        raise ValueError(f"{e_local} expert matrices, {num_experts} experts")
     if local_experts >= 0 and local_experts != e_local or weight2.qw.shape[0] != e_local:
         raise ValueError(f"{e_local} and {weight2.qw.shape[0]} expert matrices, {local_experts} local experts")
     if _mx_hip(x.payload if isinstance(x, MxRows) else x, dtype) and t:
@@ -624,9 +626,31 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
         else:
             rows = x if isinstance(x, MxRows) else _hip.mx_quantize(x, 8)
         a = _hip.mx_grouped_gate_up(rows, weight13, tiles, tile_rows, bias13, limit, alpha, src_row)
-        y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2)      # (summed in 32 bits, rounded once)
-        return _hip.mx_combine(y, topw, topi, inv, dtype, expert_start if local_experts >= 0 else 0, e_local)
+        return _mx_experts_down(a, weight2, tiles, tile_rows, bias2, topw, topi, inv, dtype, expert_start if local_experts >= 0 else 0)
     return torch_ref.mx_experts(_mx_operand(x, weight13), topw, topi, weight13, weight2, bias13, bias2, expert_start, limit, alpha)
+
+
+def _mx_experts_down(a, weight2: MxWeight, tiles, tile_rows: int, bias2, topw, topi, inv, dtype, first: int):
+    """The second product and the tokens' sums, in 32 bits and rounded once."""
+    y = _hip.mx_grouped_linear(a, weight2, tiles, tile_rows, bias2)
+    return _hip.mx_combine(y, topw, topi, inv, dtype, first, weight2.qw.shape[0])
+
+
+def mx_experts_routed(logits, x, top_k: int, renormalize: bool, weight13: MxWeight, weight2: MxWeight, bias13=None, bias2=None,
+                      expert_start: int = 0, local_experts: int = -1, limit: float = 0.0, alpha: float = 1.702):
+    """``mx_experts`` with its router's choice, the softmax over ``logits`` (``[T, E]``, or ``[splits, T, E]`` of
+    ``router_logit_partials``), on the GPU: for up to 16 rows the choice, their sort and gather are one launch."""
+    if not moe_route_small_ok(logits, x):
+        topw, topi = moe_topk(logits, top_k, renormalize)
+        return mx_experts(x, topw, topi, weight13, weight2, bias13=bias13, bias2=bias2, expert_start=expert_start,
+                          local_experts=local_experts, num_experts=logits.shape[-1], limit=limit, alpha=alpha)
+    local = weight13.qw.shape[0]
+    if weight2.qw.shape[0] != local or (local_experts >= 0 and local_experts != local) or (local_experts < 0 and logits.shape[-1] != local):
+        raise ValueError(f"{local} and {weight2.qw.shape[0]} expert matrices, {logits.shape[-1]} logits, {local_experts} local experts")
+    tile_rows = _hip.mx_tile_rows(x.shape[0] * top_k, logits.shape[-1])
+    topw, topi, inv, tiles, rows = _hip.moe_route_small(logits, x, top_k, renormalize, tile_rows, expert_start, local_experts)
+    a = _hip.mx_grouped_gate_up(_hip.mx_quantize(rows, 8), weight13, tiles, tile_rows, bias13, limit, alpha, None)
+    return _mx_experts_down(a, weight2, tiles, tile_rows, bias2, topw, topi, inv, x.dtype, expert_start if local_experts >= 0 else 0)
 
 
 def moe_align(topi, num_experts: int, tile_rows: int, expert_start: int = 0, local_experts: int = -1):
