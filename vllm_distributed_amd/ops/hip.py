@@ -2709,6 +2709,7 @@ def _mx_tiles(tiles: torch.Tensor, tile_rows: int, src: Optional[torch.Tensor], 
     if tile_rows > 16 and mx_big_ok(rows.payload.shape[0], nt, kb):
         return _mx_shape(tile_rows // 16, 4 if gated or tile_rows == 128 else 2, 1)
     assert tile_rows < 128, "tiles of 128 rows: within 32-bit byte offsets"
+    # (four waves: eight take 1.1 to 1.7 times as long for gate and up, 1.0 to 1.6 for down, with 1 to 32 rows and four kinds of experts)
     return _mx_shape(tile_rows // 16, 4, 4)
 
 
