@@ -644,8 +644,8 @@ int mx_big(const MxArgs& a, hipStream_t st) {
 template <int MT, int NT, int WM> struct MxRing {
   static constexpr int X = WM * MT * 2048, STEP = X + NT * 4096;          // bytes of a step
   static constexpr int XR = WM * (MT < 4 ? 64 : 16 * MT), SCALES = XR * 16 + NT * 1024;      // rows whose scales are loaded, bytes of a set
-  // the sets that S steps under way and the one that is multiplied may touch
-  static constexpr int sets(int steps) { return (steps + 2) / 4 + 1; }
+  // the sets that S steps under way and the one that is read may touch: S neighbouring steps, for WM 2 one more
+  static constexpr int sets(int steps) { return (steps + 1 + WM) / 4 + 1; }
   static constexpr int bytes(int steps) { return steps * STEP + sets(steps) * SCALES; }
   static constexpr int fit(int lds) { int n = 2; while (n < 8 && bytes(n + 1) <= lds) ++n; return n; }
 };
@@ -822,6 +822,7 @@ __global__ __launch_bounds__(256 * WM) void mx_ring_kernel(const MxArgs a) {
         for (int t = 0; t < NT; ++t) asm volatile("" : "+v"(acc[t][i]));    // (multiplied here, not behind the next barrier)
   }
   if (WM == 2 && wm == 0) meet();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (the zeros' loads must not outlive the LDS)
 
   // ---- lane (r, q): columns 4 q .. + 3 of tile t, row 16 i + r
   if constexpr (EPI == MX_GLU) {

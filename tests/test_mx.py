@@ -112,7 +112,11 @@ def test_refusals():
     w = quant.pack_mx(q, s)
     r = ops.mx_quantize(x)
     e3 = ops.MxWeight(w.qw.unsqueeze(0), w.ws.unsqueeze(0), 64)
+    gen = torch.Generator().manual_seed(1)
+    g1 = quant.pack_mx(*[t.unsqueeze(0) for t in oracle.random_weight(256, 128, gen)[:2]], halves=2)
+    k2 = quant.pack_mx(*[t.unsqueeze(0) for t in oracle.random_weight(64, 256, gen)[:2]])
     topw, topi = torch.ones(4, 1), torch.zeros(4, 1, dtype=torch.int32)
+    assert ops.mx_experts(x, topw, topi, g1, e3).shape == (4, 64)
     for call, error in (
             (lambda: ops.mx_quantize(x, 5), ValueError), (lambda: ops.mx_quantize(x[:, :40]), ValueError),
             (lambda: ops.mx_quantize(x[:, :0]), ValueError), (lambda: ops.mx_quantize(x.double()), TypeError),
@@ -121,11 +125,14 @@ def test_refusals():
             (lambda: ops.mx_linear(x[:, :96].contiguous().repeat(1, 3), w), ValueError),
             (lambda: ops.mx_linear(ops.mx_quantize(x, 4), w), ValueError), (lambda: ops.mx_linear(x[:, :40], w), ValueError),
             (lambda: ops.mx_gate_up(x, w), ValueError),
-            (lambda: ops.mx_experts(x, topw, topi, e3, e3, local_experts=1), ValueError),
-            (lambda: ops.mx_experts(x, topw, topi, e3, e3, local_experts=2, num_experts=4), ValueError),
-            (lambda: ops.mx_experts(x, topw, topi, e3, e3, num_experts=2), ValueError),
-            (lambda: ops.mx_experts(x[:3], topw, topi, e3, e3), ValueError),
-            (lambda: ops.mx_experts(x, topw, topi[:, :0], e3, e3), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, g1, e3, local_experts=1), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, g1, e3, local_experts=2, num_experts=4), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, g1, e3, num_experts=2), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, g1, e3, expert_start=1), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, g1, e3, expert_start=4, local_experts=1, num_experts=4), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi, g1, k2), ValueError), (lambda: ops.mx_experts(x, topw, topi, e3, e3), ValueError),
+            (lambda: ops.mx_experts(x[:3], topw, topi, g1, e3), ValueError),
+            (lambda: ops.mx_experts(x, topw, topi[:, :0], g1, e3), ValueError),
             (lambda: quant.pack_mx(q[:60], s[:60]), ValueError), (lambda: quant.pack_mx(q[:24], s[:24], halves=2), ValueError),
             (lambda: quant.pack_mx(q, s[:, :3]), ValueError), (lambda: quant.pack_mx(q.int(), s), ValueError),
             (lambda: ops.MxRows.of(r.q, r.s[:3], torch.float32), ValueError),

@@ -594,6 +594,20 @@ def mx_gate_up(x, weight: MxWeight, bias=None, limit: float = 0.0, alpha: float 
     return quant.mx_quantize(quant.mx_gated(quant.mx_product(rows, weight, bias), limit, alpha), 8, rows.dtype)
 
 
+def _mx_experts_check(weight13: MxWeight, weight2: MxWeight, expert_start: int, local_experts: int, num_experts: int) -> int:
+    """The number of matrices, which have to be the local experts', one behind the other."""
+    e = weight13.qw.shape[0]
+    if weight13.rows % 256 or weight13.rows // 256 != weight2.qw.shape[-3]:
+        raise ValueError(f"{weight13.rows} rows of gate and up (halves of whole 128 are wanted) and {weight2.qw.shape[-3] * 128} columns of down")
+    if weight2.qw.shape[0] != e or (local_experts >= 0 and local_experts != e):
+        raise ValueError(f"{e} and {weight2.qw.shape[0]} expert matrices, {local_experts} local experts")
+    if local_experts >= 0 and (not num_experts or not 0 <= expert_start <= num_experts - local_experts):
+        raise ValueError(f"local experts {expert_start} .. {expert_start + local_experts - 1} of {num_experts}: the number of the router's outputs is wanted")
+    if local_experts < 0 and (num_experts not in (0, e) or expert_start):
+        raise ValueError(f"{e} expert matrices from {expert_start} on, {num_experts} experts: local_experts is wanted")
+    return e
+
+
 def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None, bias2=None, expert_start: int = 0,
                local_experts: int = -1, num_experts: int = 0, limit: float = 0.0, alpha: float = 1.702):
     """A sparse block behind its router: ``sum_j topw[t, j] down_e(gated_e(x[t]))``, ``e = topi[t, j]``, for experts whose matrices are
@@ -601,7 +615,7 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
     16-bit rows or an ``MxRows``, ``topw [T, k]`` fp32, ``topi [T, k]`` int32.  ``expert_start`` / ``local_experts`` (expert parallel): the
     matrices are those of experts ``expert_start ..``; ``num_experts``: the router's outputs then.  Slots of other numbers (-1: nobody) add
     nothing."""
-    e_local = weight13.qw.shape[0]
+    e_local = _mx_experts_check(weight13, weight2, expert_start, local_experts, num_experts)
     total = num_experts or (e_local if local_experts < 0 else expert_start + local_experts)
     t, k = topi.shape
     width = x.width if isinstance(x, MxRows) else x.shape[-1]
@@ -610,12 +624,6 @@ def mx_experts(x, topw, topi, weight13: MxWeight, weight2: MxWeight, bias13=None
     if len(x.shape) != 2 or x.shape[0] != t or topw.shape != topi.shape:
         raise ValueError(f"rows {tuple(x.shape)}, choices {tuple(topi.shape)}, weights {tuple(topw.shape)}")
     dtype = x.dtype
-    if local_experts >= 0 and not num_experts:
-        raise ValueError("the number of the router's outputs is wanted beside local_experts")
-    if local_experts < 0 and num_experts not in (0, e_local):
-        raise ValueError(f"{e_local} expert matrices, {num_experts} experts")
-    if local_experts >= 0 and local_experts != e_local or weight2.qw.shape[0] != e_local:
-        raise ValueError(f"{e_local} and {weight2.qw.shape[0]} expert matrices, {local_experts} local experts")
     if _mx_hip(x.payload if isinstance(x, MxRows) else x, dtype) and t:
         tile_rows = _hip.mx_tile_rows(t * k, total)
         if tile_rows > 64 and not (_hip.mx_sorted_ok(t * k, weight13) and _hip.mx_sorted_ok(t * k, weight2)):
@@ -644,9 +652,7 @@ def mx_experts_routed(logits, x, top_k: int, renormalize: bool, weight13: MxWeig
         topw, topi = moe_topk(logits, top_k, renormalize)
         return mx_experts(x, topw, topi, weight13, weight2, bias13=bias13, bias2=bias2, expert_start=expert_start,
                           local_experts=local_experts, num_experts=logits.shape[-1], limit=limit, alpha=alpha)
-    local = weight13.qw.shape[0]
-    if weight2.qw.shape[0] != local or (local_experts >= 0 and local_experts != local) or (local_experts < 0 and logits.shape[-1] != local):
-        raise ValueError(f"{local} and {weight2.qw.shape[0]} expert matrices, {logits.shape[-1]} logits, {local_experts} local experts")
+    _mx_experts_check(weight13, weight2, expert_start, local_experts, logits.shape[-1])
     tile_rows = _hip.mx_tile_rows(x.shape[0] * top_k, logits.shape[-1])
     topw, topi, inv, tiles, rows = _hip.moe_route_small(logits, x, top_k, renormalize, tile_rows, expert_start, local_experts)
     a = _hip.mx_grouped_gate_up(_hip.mx_quantize(rows, 8), weight13, tiles, tile_rows, bias13, limit, alpha, None)
