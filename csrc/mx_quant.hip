@@ -6,14 +6,30 @@
 
 namespace {
 
+// A thread's groups of 8 columns: row and place in it, a grid apart.  One division in front of the loop (one for each group: 28672 x 4096
+// to 4 bits and back 132 us instead of 130)
+struct MxWalk {
+  long row, rows_on;
+  int c, c_on, per_row;
+  __device__ __forceinline__ MxWalk(long i, long stride, int per) : row(i / per), rows_on(stride / per), c((int)(i - row * per)),
+                                                                    c_on((int)(stride - rows_on * per)), per_row(per) {}
+  __device__ __forceinline__ void next() {
+    row += rows_on;
+    c += c_on;
+    if (c >= per_row) { c -= per_row; ++row; }
+  }
+};
+
 // rows of x [M][K] (src: x[src[row]]) -> q [M][width of BITS], s [M][.]; columns K .. Kp are zeros
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s, long lds,
                                                           const T* __restrict__ x, long ldx, long groups, int per_row, int K,
                                                           const int* __restrict__ src, int x_rows) {
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < groups; i += gridDim.x * 256L) {
-    const long row = i / per_row;
-    const int c = (int)(i - row * per_row);
+  const long stride = gridDim.x * 256L;
+  long i = blockIdx.x * 256L + threadIdx.x;
+  for (MxWalk w(i, stride, per_row); i < groups; i += stride, w.next()) {
+    const long row = w.row;
+    const int c = w.c;
     float v[8];
     if (8 * c < K) {                              // (whole blocks: a quad agrees)
       mx_load8(x + (src != nullptr ? (long)min(max(src[row], 0), x_rows - 1) : row) * ldx + 8 * c, v);
@@ -53,9 +69,11 @@ __device__ __forceinline__ float mx_scaled(float v, uint32_t byte) {
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ q, long ldq,
                                                             const uint8_t* __restrict__ s, long lds, long groups, int per_row) {
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < groups; i += gridDim.x * 256L) {
-    const long row = i / per_row;
-    const int c = (int)(i - row * per_row);
+  const long stride = gridDim.x * 256L;
+  long i = blockIdx.x * 256L + threadIdx.x;
+  for (MxWalk at(i, stride, per_row); i < groups; i += stride, at.next()) {
+    const long row = at.row;
+    const int c = at.c;
     const uint32_t byte = s[row * lds + (c >> 2)];
     float v[8];
     if constexpr (BITS == 8) {
