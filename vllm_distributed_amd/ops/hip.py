@@ -2635,10 +2635,10 @@ def mx_operand(x: torch.Tensor, kb: int):
 def mx_linear(x, w: quant.MxWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     _, nt, kb = _mx_check(x, w, bias, False)
     m, n, dev = x.shape[0], w.rows, x.device
-    out = torch.empty((m, n), dtype=x.dtype, device=dev)
+    out = torch.empty(m, n, dtype=x.dtype, device=dev)
     if m:
         plan = mx_plan(m, n, kb, mx_big_ok(m, nt, kb))
-        partial = torch.empty((plan[1], m, n), dtype=torch.float32, device=dev) if plan[1] > 1 else None
+        partial = torch.empty(plan[1], m, n, dtype=torch.float32, device=dev) if plan[1] > 1 else None
         _mx_gemm(0, x, w, 1, kb, bias, out, n, None, 0, partial, plan)
     return out
 
@@ -2656,7 +2656,7 @@ def mx_linear_partials(x, w: quant.MxWeight) -> Optional[torch.Tensor]:
     plan = mx_plan(m, n, kb, mx_big_ok(m, nt, kb)) if m else (0, 1)
     if plan[1] == 1:
         return None
-    partial = torch.empty((plan[1], m, n), dtype=torch.float32, device=x.device)
+    partial = torch.empty(plan[1], m, n, dtype=torch.float32, device=x.device)
     _mx_gemm(1, x, w, 1, kb, None, None, 0, None, 0, partial, plan)
     return partial
 
@@ -2672,7 +2672,7 @@ def mx_gate_up(x, w: quant.MxWeight, bias: Optional[torch.Tensor], limit: float,
     r = _mx_gated_out(x, w, m)
     if m:
         plan = mx_plan(m, w.rows, kb, mx_big_ok(m, nt, kb), True)
-        partial = torch.empty((plan[1], m, w.rows), dtype=torch.float32, device=x.device) if plan[1] > 1 else None
+        partial = torch.empty(plan[1], m, w.rows, dtype=torch.float32, device=x.device) if plan[1] > 1 else None
         _mx_gemm(2, x, w, 1, kb, bias, r.payload, r.payload.shape[1], r.scales, r.scales.shape[1], partial, plan, limit, alpha)
     return r
 
@@ -2719,7 +2719,7 @@ def mx_grouped_linear(rows: quant.MxRows, w: quant.MxWeight, tiles: torch.Tensor
     stay unwritten."""
     groups, nt, kb = _mx_check(rows, w, bias, True)
     mt = _mx_tiles(tiles, tile_rows, None, rows, nt, kb, False)
-    out = torch.empty((rows.shape[0], w.rows), dtype=torch.float32, device=rows.device)
+    out = torch.empty(rows.shape[0], w.rows, dtype=torch.float32, device=rows.device)
     if out.shape[0]:
         _mx_gemm(1, rows, w, groups, kb, bias, None, w.rows, None, 0, out, (mt, 1), tiles=tiles)
     return out
@@ -2734,7 +2734,7 @@ def mx_combine(y: torch.Tensor, topw: torch.Tensor, topi: torch.Tensor, inv: tor
     assert topw.dtype == torch.float32 and topw.is_contiguous() and topw.shape == topi.shape
     assert topi.dtype == torch.int32 and topi.is_contiguous() and inv.dtype == torch.int32 and inv.is_contiguous()
     _mx_device(y.get_device(), topw, topi, inv)
-    out = torch.empty((t, h), dtype=dtype, device=y.device)
+    out = torch.empty(t, h, dtype=dtype, device=y.device)
     _check(_LIB.vdamd_mx_combine(out.data_ptr(), y.data_ptr(), topw.data_ptr(), topi.data_ptr(), inv.data_ptr(), t, k, h, expert_start,
                                  local_experts, _DT[dtype], _stream()), "mx_combine")
     return out

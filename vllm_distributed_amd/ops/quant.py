@@ -235,9 +235,10 @@ class MxRows:
         if width <= 0 or width % MX_BLOCK:
             raise ValueError(f"{width} columns are not whole blocks of {MX_BLOCK}")
         kp = (width + 127) // 128 * 128
-        payload = (torch.empty((rows, kp), dtype=torch.float8_e4m3fn, device=device) if bits == 8
-                   else torch.empty((rows, kp // 2), dtype=torch.uint8, device=device))
-        return MxRows(payload, torch.empty((rows, (kp + 511) // 512 * 16), dtype=torch.float8_e8m0fnu, device=device), width, bits, dtype)
+        # (sizes as numbers: a tuple of them takes torch half as long again, 1.6 us)
+        payload = (torch.empty(rows, kp, dtype=torch.float8_e4m3fn, device=device) if bits == 8
+                   else torch.empty(rows, kp // 2, dtype=torch.uint8, device=device))
+        return MxRows(payload, torch.empty(rows, (kp + 511) // 512 * 16, dtype=torch.float8_e8m0fnu, device=device), width, bits, dtype)
 
     @staticmethod
     def of(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> "MxRows":
