@@ -91,7 +91,8 @@ class GptOssMoE(FusedMoE):
         spec = active_quant()
         self.microscaled = spec is not None and spec.method == "mxfp4"
         if self.microscaled and (H % 32 or I % 32 or E > 512 or self.top_k > 16):
-            logger.warning("experts of %d x %d on each rank do not divide into blocks of 32: they are kept in %s", H, I, dtype)
+            logger.warning("%d experts of %d x %d on each rank, top %d, are kept in %s: whole blocks of 32, at most 512 experts and 16 choices "
+                           "are microscaled", E, H, I, self.top_k, dtype)
             self.microscaled = False
         if self.microscaled:
             del self.w13, self.w2           # in their place the matrices as blocks, [expert][kind], until they are packed
