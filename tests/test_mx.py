@@ -141,6 +141,31 @@ def test_refusals():
             call()
 
 
+def one_row_views(dtype):
+    """[1, 64] views whose row stride torch leaves as it was: rows of a matrix 523 wide from the front, the middle and an odd address, a column
+    turned, an expanded row, a part of a longer row, and leading dimensions."""
+    base = rows(5, 523, dtype=dtype)
+    column = rows(64, 1, dtype=dtype)
+    return [base[:1, :64], base[1:2, 5:69], base[4:, 8:72], column.t(), column.flatten().expand(1, 64), base[:1].as_strided((1, 64), (0, 1)),
+            base[2:3, :128:2], base[3:4, None, :64]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_row_of_any_stride_is_a_row(dtype):
+    """What the kernels get: rows at 16-byte borders, their stride a multiple of eight that holds them, however many there are."""
+    from vllm_distributed_amd.ops import hip
+    views = one_row_views(dtype)
+    assert len({v.stride() for v in views}) > 3
+    base = rows(6, 523, dtype=dtype)
+    for x in views + [base[:, :64], base[::2, 3:67], base[:1, :64].expand(3, 64), base[:0, :64]]:
+        got = hip._mx_rows(x)
+        assert torch.equal(got, x.reshape(-1, 64))
+        if got.shape[0]:
+            assert got.stride(1) == 1 and got.stride(0) % 8 == 0 and got.stride(0) >= 64 and got.data_ptr() % 16 == 0, (x.stride(), got.stride())
+    keep = base.new_zeros(3, 72)[:1, :64]                        # (nothing is copied that can be read as it is)
+    assert hip._mx_rows(keep).data_ptr() == keep.data_ptr()
+
+
 # ------------------------------------------------------------------ layers and models
 def q8(x):
     return oracle.blocks(x.reshape(-1, x.shape[-1]), 8)[2].view(x.shape)

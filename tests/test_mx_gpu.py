@@ -106,6 +106,37 @@ def test_quantize_strides_and_borders():
     assert ops.mx_dequantize(ops.mx_quantize(base[:0, :64])).shape == (0, 64)
 
 
+@pytest.mark.parametrize("at", range(8))
+def test_one_row_of_any_stride(at):
+    """One row that is a view: quantised, normed, multiplied, gated and through experts like its copy."""
+    from tests.test_mx import one_row_views
+    from vllm_distributed_amd import ops
+    x = one_row_views(torch.bfloat16)[at]
+    flat = x.reshape(1, 64).clone(memory_format=torch.contiguous_format)
+    # (the same view of the same numbers on the device: a whole storage moves, strides and offset stay)
+    base = torch.empty(0, dtype=x.dtype, device="cuda").set_(x.untyped_storage().cuda(), x.storage_offset(), x.shape, x.stride())
+    assert base.stride() == x.stride() and torch.equal(base.cpu(), x)
+    whole = flat.cuda()
+    gain, residual = torch.ones(64, dtype=x.dtype).cuda(), rows(1, 64).cuda()
+    w, _ = make(40, 64)
+    w13, _ = make(256, 64, halves=2)
+    e13, _ = make_experts(2, 256, 64, halves=2)
+    e2, _ = make_experts(2, 64, 128)
+    topi, topw = torch.tensor([[1, 0]], dtype=torch.int32).cuda(), torch.tensor([[0.75, 0.25]]).cuda()
+    logits = torch.tensor([[0.5, -1.0]]).cuda()
+
+    def bits(out):
+        flat = [out] if isinstance(out, (torch.Tensor, ops.MxRows)) else list(out)
+        parts = [t for o in flat for t in ((o.payload.view(torch.uint8), o.s.view(torch.uint8)) if isinstance(o, ops.MxRows) else (o,))]
+        return [t.reshape(1, -1) for t in parts]
+    calls = [lambda v: ops.mx_quantize(v, 8), lambda v: ops.mx_quantize(v, 4), lambda v: ops.rms_norm_mx(v, gain, 1e-5),
+             lambda v: ops.fused_add_rms_norm_mx(v, residual, gain, 1e-5), lambda v: ops.mx_linear(v, w), lambda v: ops.mx_gate_up(v, w13)]
+    if x.dim() == 2:
+        calls += [lambda v: ops.mx_experts(v, topw, topi, e13, e2), lambda v: ops.mx_experts_routed(logits, v, 2, True, e13, e2)]
+    for call in calls:
+        assert all(torch.equal(a, b) for a, b in zip(bits(call(base)), bits(call(whole))))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_dequantize_every_code(dtype):
     from vllm_distributed_amd import ops

@@ -2448,10 +2448,13 @@ def _mx_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
 
 
 def _mx_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` as rows that the kernels can read: unit stride, 16-byte borders."""
+    """``x`` as rows that the kernels can read: unit stride, 16-byte borders, whatever the stride of a single row was."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    m, k = x2.shape
     s0, s1 = x2.stride()
-    if s1 != 1 or s0 % 8 or s0 < x2.shape[1] or x2.data_ptr() % 16:
+    if m == 1 and s0 != k:            # (one row's stride means nothing to torch: contiguous() and clone() keep it)
+        x2, s0 = x2.as_strided((1, k), (k, s1)), k
+    if s1 != 1 or s0 % 8 or s0 < k or x2.data_ptr() % 16:
         x2 = x2.contiguous()
         if x2.data_ptr() % 16:
             x2 = x2.clone()
