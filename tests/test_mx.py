@@ -1,6 +1,7 @@
 """Microscaled rows, weights and layers on the CPU: the definition against 64 bits, the layout, refusals, and models whose layers are
 microscaled (``--quantization mxfp4``)."""
 import json
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -164,6 +165,25 @@ def test_one_row_of_any_stride_is_a_row(dtype):
             assert got.stride(1) == 1 and got.stride(0) % 8 == 0 and got.stride(0) >= 64 and got.data_ptr() % 16 == 0, (x.stride(), got.stride())
     keep = base.new_zeros(3, 72)[:1, :64]                        # (nothing is copied that can be read as it is)
     assert hip._mx_rows(keep).data_ptr() == keep.data_ptr()
+
+
+def test_norm_kernel_gets_operands_at_16_byte_borders(monkeypatch):
+    """A branch or a residual from an odd address is copied; one that can be read as it is is not."""
+    from vllm_distributed_amd.ops import hip
+    seen = []
+    monkeypatch.setattr(hip, "_LIB", SimpleNamespace(vdamd_mx_rms_norm=lambda *a: seen.append(a) or 0))
+    monkeypatch.setattr(hip, "_mx_device", lambda *a: None)
+    monkeypatch.setattr(hip, "_stream", lambda: 0)
+    m, h = 3, 64
+    gain = torch.ones(h, dtype=torch.bfloat16)
+    flat = rows(1, (m + 1) * h, dtype=torch.bfloat16).flatten()
+    for at in (0, 1, 4, 8):
+        x, residual = flat[8:8 + m * h].view(m, h), flat[at:at + m * h].view(m, h)
+        _, out = hip.mx_rms_norm(x, None, residual, gain, 1e-5)
+        # (the C entry's order: q, ldq, s, lds, residual_out, x, ldx, slabs, ks, residual, ..)
+        q, residual_out, x_at, residual_at = (seen[-1][i] for i in (0, 4, 5, 9))
+        assert not (q | residual_out | x_at | residual_at) % 16
+        assert (residual_at == residual.data_ptr()) == (at % 8 == 0) and out.shape == residual.shape
 
 
 # ------------------------------------------------------------------ layers and models

@@ -208,6 +208,20 @@ def test_norm_keeps_its_inputs_and_takes_strides():
     assert torch.equal(r.payload.view(torch.uint8), again.payload.view(torch.uint8)) and torch.equal(r.s.view(torch.uint8), again.s.view(torch.uint8)) and torch.equal(out, out2)
 
 
+@pytest.mark.parametrize("at", [1, 4, 8])
+def test_norm_of_a_residual_from_any_address(at):
+    from vllm_distributed_amd import ops
+    m, h = 3, 96
+    flat = rows(1, (m + 1) * h).flatten().cuda()
+    x, residual, gain = rows(m, h).cuda(), flat[at:at + m * h].view(m, h), (1 + 0.2 * torch.randn(h)).to(torch.bfloat16).cuda()
+    slabs = torch.randn(2, m, h).cuda()
+    before = flat.clone()
+    for call in (lambda r: ops.fused_add_rms_norm_mx(x, r, gain, 1e-5), lambda r: ops.reduce_add_rms_norm_mx(slabs, r, gain, 1e-5)):
+        (a, sa), (b, sb) = call(residual), call(residual.clone())
+        assert torch.equal(sa, sb) and torch.equal(a.payload.view(torch.uint8), b.payload.view(torch.uint8))
+        assert torch.equal(a.s.view(torch.uint8), b.s.view(torch.uint8)) and torch.equal(flat, before)
+
+
 # ------------------------------------------------------------------ products
 def make(n, k, halves=1, spread=3):
     from vllm_distributed_amd.ops import quant

@@ -2507,6 +2507,8 @@ def mx_rms_norm(x: Optional[torch.Tensor], slabs: Optional[torch.Tensor], residu
     if residual is not None:
         assert residual.dtype == dtype and residual.numel() == m * h and residual.shape[-1] == h
         residual = residual.contiguous()
+        if residual.data_ptr() % 16:
+            residual = residual.clone()
         out = torch.empty_like(residual)
     _mx_device(dev, x2, slabs, residual)
     r = quant.MxRows.empty(m, h, 8, dtype, weight.device)
