@@ -306,6 +306,77 @@ def test_every_shape_of_the_ring(m, n, k, mt, nt, ksplit, monkeypatch):
         check_rows(ops.mx_gate_up(xr, w), v, slack)
 
 
+BIG_TILES = [(1, 8, 32), (255, 264, 128), (256, 256, 1056), (257, 1000, 160), (2049, 2568, 384), (300, 1000, 1184), (2049, 9992, 288)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", BIG_TILES)
+def test_large_tiles(m, n, k, dtype, monkeypatch):
+    """The kernel of 256-row tiles at rows, columns and steps that leave parts of a tile empty: one step, an odd number of them, columns of one
+    die alone, and (the last) more tiles than workgroups, so that loads run on into the next one."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    monkeypatch.setattr(hip, "mx_plan", lambda *a: (hip.MX_BIG, 1))
+    x = (rows(m, k).float() / 8).to(dtype)
+    w, wv = make(n, k, spread=1)
+    bias = torch.randn(n).to(dtype)
+    xr, xv = ops.mx_quantize(x.cuda()), oracle.blocks(x, 8)[2]
+    check_product(ops.mx_linear(xr, w, bias.cuda()), xv, wv, dtype, bias)
+    check_product(ops.mx_linear(xr, w), xv, wv, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,inter,k,limit", [(1, 128, 32, 0.0), (255, 384, 160, 7.0), (513, 1408, 288, 0.0), (2049, 256, 128, 7.0),
+                                             (300, 128, 1184, 0.0), (2049, 3200, 288, 7.0)])
+def test_gated_large_tiles(m, inter, k, limit, dtype, monkeypatch):
+    """Likewise the gated product, whose tiles have columns of both halves."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    monkeypatch.setattr(hip, "mx_plan", lambda *a: (hip.MX_BIG, 1))
+    x = (rows(m, k, spread=0.3).float() / k ** 0.5).to(dtype)
+    w, wv = make(2 * inter, k, halves=2, spread=1)
+    bias = torch.randn(2 * inter).to(dtype)
+    for b in (bias, None):
+        r = ops.mx_gate_up(ops.mx_quantize(x.cuda()), w, None if b is None else b.cuda(), limit=limit)
+        check_rows(r, *gated_slack(oracle.blocks(x, 8)[2], wv, b, limit))
+
+
+@pytest.mark.parametrize("mt,nt,ksplit", [(2, 2, 2), (4, 2, 3), (8, 4, 2), (8, 4, 3)])
+@pytest.mark.parametrize("m,inter,k,limit", [(33, 256, 1056, 0.0), (130, 640, 544, 7.0)])
+def test_gated_products_of_a_split_reduction(m, inter, k, limit, mt, nt, ksplit, monkeypatch):
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    monkeypatch.setattr(hip, "mx_plan", lambda *a: (hip._mx_shape(mt, nt, 1), ksplit))
+    x = (rows(m, k, spread=0.3).float() / k ** 0.5).to(torch.bfloat16)
+    w, wv = make(2 * inter, k, halves=2, spread=1)
+    b = torch.randn(2 * inter).to(torch.bfloat16)
+    check_rows(ops.mx_gate_up(x.cuda(), w, b.cuda(), limit=limit), *gated_slack(oracle.blocks(x, 8)[2], wv, b, limit))
+
+
+@pytest.mark.parametrize("m,n,k,gated,shape", [
+    (2, 1000, 288, False, (1, 1, 8)), (7, 1000, 288, False, (1, 1, 8)), (3, 4104, 160, False, (1, 2, 8)), (13, 4104, 160, False, (1, 2, 8)),
+    (2, 16424, 160, False, (1, 2, 8)), (3, 16424, 160, False, (1, 4, 4)), (9, 16424, 160, False, (1, 4, 4)), (4, 64, 11520, False, (1, 1, 8)),
+    (1, 512, 288, True, (1, 4, 8)), (11, 512, 288, True, (1, 4, 8)), (4, 256, 11520, True, (1, 4, 8)), (4, 16384, 160, True, (1, 4, 4)),
+    (12, 16384, 160, True, (1, 4, 4))])
+def test_every_shape_of_the_stream(m, n, k, gated, shape):
+    """Every launch of the streaming kernel that the plan makes, at sizes where it makes it: up to four rows are quantised inside (11520
+    columns: as many as fit, next to the sums of eight waves), others in front."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    kb = (k + 127) // 128
+    assert hip.mx_plan(m, n, kb, True, gated) == (hip._mx_shape(*shape), 1) and hip.mx_fused_ok(m, kb) == (m <= 4)
+    x = (rows(m, k, spread=0.3).float() / k ** 0.5).to(torch.bfloat16)
+    w, wv = make(n, k, halves=2 if gated else 1, spread=1)
+    b = torch.randn(n).to(torch.bfloat16)
+    xv = oracle.blocks(x, 8)[2]
+    for bias in (b, None):
+        on_gpu = None if bias is None else bias.cuda()
+        if gated:
+            check_rows(ops.mx_gate_up(x.cuda(), w, on_gpu), *gated_slack(xv, wv, bias, 0.0))
+        else:
+            check_product(ops.mx_linear(x.cuda(), w, on_gpu), xv, wv, torch.bfloat16, bias)
+
+
 @pytest.mark.parametrize("m", [17, 40, 130])
 def test_operands_past_32_bit_offsets_stream(m, monkeypatch):
     """What runs for operands of 4 GiB and more, at small ones."""
@@ -474,6 +545,24 @@ def test_experts(t, e, k, h, inter, limit):
     y = ops.mx_experts(x.cuda(), topw.cuda(), topi.cuda(), w13, w2, None if b13 is None else quant.pad_mx_bias(b13, 2).cuda(),
                        None if b2 is None else b2.cuda(), limit=limit)
     want, bound = expert_block(oracle.blocks(x, 8)[2], topw, topi, v13, v2, b13, b2, limit)
+    off = (y.cpu().double() - want).abs()
+    assert (off <= bound).all(), f"worst {(off / bound).max():.3g} of the bound"
+    assert off.norm() <= 2.0 ** -6 * want.norm()
+
+
+def test_experts_of_more_outputs_than_workgroups():
+    """256-row tiles, 24 of them by 11 columns: loads run on from one expert's output into the next one's."""
+    from vllm_distributed_amd import ops
+    from vllm_distributed_amd.ops import hip
+    t, e, k, h, inter = 2800, 8, 2, 160, 1408
+    assert hip.mx_tile_rows(t * k, e) == 256
+    x = (rows(t, h, spread=0.3).float() / h ** 0.5).to(torch.bfloat16)
+    w13, v13 = make_experts(e, 2 * inter, h, halves=2)
+    w2, v2 = make_experts(e, h, inter)
+    topi = torch.stack([torch.randperm(e)[:k] for _ in range(t)]).int()
+    topw = torch.rand(t, k)
+    y = ops.mx_experts(x.cuda(), topw.cuda(), topi.cuda(), w13, w2)
+    want, bound = expert_block(oracle.blocks(x, 8)[2], topw, topi, v13, v2, None, None, 0.0)
     off = (y.cpu().double() - want).abs()
     assert (off <= bound).all(), f"worst {(off / bound).max():.3g} of the bound"
     assert off.norm() <= 2.0 ** -6 * want.norm()
