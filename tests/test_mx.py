@@ -186,6 +186,35 @@ def test_norm_kernel_gets_operands_at_16_byte_borders(monkeypatch):
         assert (residual_at == residual.data_ptr()) == (at % 8 == 0) and out.shape == residual.shape
 
 
+@pytest.mark.parametrize("m", [1, 256, 2000, 4096, 8131, 12288, 20000])
+def test_large_tiles_are_expected_to_take_the_rounds_that_they_take(m):
+    """The plan's expected time of 256-row tiles against the launch, dealt out as the kernel does: eight dies, each with its own tile columns
+    and at most 32 workgroups, one tile after the other."""
+    from vllm_distributed_amd.ops import hip
+    for n in (8, 264, 512, 1000, 1280, 2880, 4104, 5120, 6144, 10240, 57344):
+        for kb in (1, 9, 64):
+            ntm, ntn = (m + 255) // 256, (n + 255) // 256
+            per_die = min(ntm * ((ntn + 7) // 8), 32)
+            tiles = [ntm * ((ntn * (d + 1) >> 3) - (ntn * d >> 3)) for d in range(8)]
+            rounds = max(len(range(i, t, per_die)) for t in tiles for i in range(per_die))
+            got = hip._mx_estimate(m, n, kb, hip.MX_BIG, 0, 1)
+            # (a step 1 us, 1.22 on a full chip, 5.4 beside the steps of a tile)
+            assert rounds * (kb + 5.4) - 1e-6 <= got <= rounds * (1.22 * kb + 5.4) + 1e-6, (n, kb, rounds, got)
+
+
+def test_narrow_outputs_of_many_rows_go_through_the_ring():
+    """Fewer than eight tile columns leave dies without work: us of large tiles and of the ring beside each size."""
+    from vllm_distributed_amd.ops import hip
+    for m, n, k, gated in ((12288, 1280, 8192, False),      # 184, 129
+                           (20000, 264, 4640, False),       # 150, 63
+                           (16384, 1000, 1056, False),      # 48, 38
+                           (12288, 768, 4096, False),       # 92, 62
+                           (6000, 5120, 6144, True)):       # 200, 189
+        assert hip.mx_plan(m, n, (k + 127) // 128, True, gated)[0] != hip.MX_BIG, (m, n, k)
+    for m, n, k, gated in ((4096, 8192, 28672, False), (4096, 2880, 4096, False), (8192, 6144, 4096, False), (6007, 28672, 4096, True)):
+        assert hip.mx_plan(m, n, (k + 127) // 128, True, gated) == (hip.MX_BIG, 1), (m, n, k)
+
+
 # ------------------------------------------------------------------ layers and models
 def q8(x):
     return oracle.blocks(x.reshape(-1, x.shape[-1]), 8)[2].view(x.shape)
