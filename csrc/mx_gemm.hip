@@ -738,8 +738,7 @@ __global__ __launch_bounds__(256 * WM) void mx_ring_kernel(const MxArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int swz = (r >> 1) & 7, so0 = (q ^ swz) << 4, so1 = ((4 + q) ^ swz) << 4;
-  // set of four steps ss: (ss - first) mod SETS; a step's buffer: (k - lo) mod S
-  const int first = lo >> 2;
+  // set of four steps ss: (ss - lo / 4) mod SETS; a step's buffer: (k - lo) mod S
   auto issue_scales = [&](int k) {
     if (k < hi && (k == lo || (k & 3) == 0)) {
       stage_scales(k >> 2, sset);
