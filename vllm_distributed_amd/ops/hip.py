@@ -2579,10 +2579,12 @@ def _mx_estimate(m: int, n: int, kb: int, mt: int, nt: int, ksplit: int, gated: 
     """Expected us of a product; ``mt`` ``MX_BIG``: 256-row tiles, whose steps slow down as they fill the chip."""
     if mt == MX_BIG:
         # (us of large tiles and of the ring where there are fewer tile columns than dies: 12288 rows of 8192 into 1280 184 and 129, 20000 of
-        # 4640 into 264 150 and 63.  With the rounds of both kernels as they are, and 5 us more for the gate of each, the choice for 144
-        # products of 300 to 30000 rows is 1 % behind the best on average, 16 % at worst; counting tiles alone it was 8 %, and 2.5 times)
+        # 4640 into 264 150 and 63.  A die with one column shares no rows of x between its units: 1.4 us a step on more than 128 of them.
+        # With the rounds of both kernels as they are, and 4.5 us more for the gate of each, the choice for 144 products of 300 to 30000
+        # rows is 0.3 % behind the best on average, 11 % at worst; counting tiles alone it was 8 %, and 2.5 times)
         tiles, rounds = _mx_big_rounds(m, n)
-        return rounds * (kb * (1.0 + 0.22 * min(1.0, max(0.0, (tiles - 128) / 128))) + (10.4 if gated else 5.4))
+        slower = 0.4 * min(1.0, max(0.0, (tiles - 128) / 32)) if n <= 2048 else 0.22 * min(1.0, max(0.0, (tiles - 128) / 128))
+        return rounds * (kb * (1.0 + slower) + (9.9 if gated else 5.4))
     load = -(-n // (64 * nt)) * -(-m // (16 * mt)) * ksplit / 256
     alone, shared = _MX_RING[mt, nt]
     # (workgroups of 128 rows have a unit to themselves: in rounds, each with a ring to fill and results to store, 4 us)
